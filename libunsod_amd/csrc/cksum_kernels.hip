@@ -49,6 +49,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <tuple>
 #include <vector>
 
 #include "mi_cksum.h"
@@ -2309,37 +2310,40 @@ uint32_t batch_max_len(const mi_pkt_batch *b) {
   return b->max_len ? b->max_len : 1500u;
 }
 
-int launched() {
-  HIP_TRY(hipGetLastError());
-  return 0;
-}
-
-// Events the NEXT verify launch of this thread carries in its own dispatch
+// Events the NEXT launch of this thread carries in its own dispatch
 // (hipExtLaunchKernel start / stop events: no separate marker packets, so the
 // region's first kernel is not queued behind one and completion is the
-// kernel's own signal).  Set by mi_cksum_repeat_run, consumed by VLAUNCH.
+// kernel's own signal).  Set by mi_cksum_repeat_run, consumed by launch().
 struct LaunchEv {
   hipEvent_t start = nullptr, stop = nullptr;
 };
 thread_local LaunchEv t_lev;
-#define VLAUNCH(K, GRID, BLOCK, SHM, S, ...)                                                         \
-  do {                                                                                               \
-    if (t_lev.start || t_lev.stop) {                                                                 \
-      const LaunchEv ev_ = t_lev;                                                                    \
-      t_lev = LaunchEv();                                                                            \
-      hipExtLaunchKernelGGL(K, GRID, BLOCK, SHM, S, ev_.start, ev_.stop, 0, __VA_ARGS__);            \
-    } else {                                                                                         \
-      hipLaunchKernelGGL(K, GRID, BLOCK, SHM, S, __VA_ARGS__);                                       \
-    }                                                                                                \
-  } while (0)
+// Launch kernel k(a...) on s, no dynamic LDS.  The result is the launch call's
+// own: kernel<<<>>> returns nothing, and the thread's last error
+// (hipGetLastError) may be one an earlier call left, here or in the caller's
+// code -- the kernel would be reported as failed with its stores under way.
+template <typename... P, typename... A>
+int launch(void (*k)(P...), dim3 grid, dim3 block, hipStream_t s, A... a) {
+  std::tuple<P...> p(a...);
+  const LaunchEv ev = t_lev;
+  t_lev = LaunchEv();
+  const hipError_t e = std::apply(
+      [&](auto &...v) {
+        void *args[] = {(void *)&v...};
+        return ev.start || ev.stop ? hipExtLaunchKernel((const void *)k, grid, block, args, 0, s, ev.start, ev.stop, 0)
+                                   : hipLaunchKernel((const void *)k, grid, block, args, 0, s);
+      },
+      p);
+  if (e != hipSuccess) return set_err(-EIO, "kernel launch: %s", hipGetErrorString(e));
+  return 0;
+}
 
 int launch_verify_shape(const Desc &d, Shape sh, uint16_t *ip, uint16_t *l4, uint8_t *st,
                         uint32_t *bad, hipStream_t s) {
   const int grid = grid_for(d.n, sh.g);
 #define X(G_, U_)                                                                        \
   if (sh.g == G_ && sh.u == U_) {                                                        \
-    VLAUNCH((k_ipv4_verify<G_, U_>), dim3(grid), dim3(kBlock), 0, s, d, ip, l4, st, bad);   \
-    return launched();                                                                   \
+    return launch(k_ipv4_verify<G_, U_>, dim3(grid), dim3(kBlock), s, d, ip, l4, st, bad); \
   }
   FOR_GU(X)
 #undef X
@@ -2579,8 +2583,7 @@ int launch_verify(const Desc &d, uint32_t max_len, uint16_t *ip, uint16_t *l4, u
     jnote("  deal counters", deal, kDealSetBytes, dblocks);
 #define X(G_, U_)                                                                                              \
   if (pl.shape.g == G_ && pl.shape.u == U_) {                                                                  \
-    VLAUNCH((k_ipv4_verify_dyn<G_, U_>), dim3(dblocks), dim3(kBlock), 0, s, d, ip, l4, st, bad, deal);           \
-    return launched();                                                                                         \
+    return launch(k_ipv4_verify_dyn<G_, U_>, dim3(dblocks), dim3(kBlock), s, d, ip, l4, st, bad, deal);        \
   }
     MI_DEAL_SHAPES(X)
 #undef X
@@ -2591,8 +2594,7 @@ int launch_verify(const Desc &d, uint32_t max_len, uint16_t *ip, uint16_t *l4, u
   if (pl.kind == kPlanRun && pl.dma) {
 #define X(U_, R_)                                                                                            \
   if (pl.dma == 10 * U_ + R_) {                                                                              \
-    VLAUNCH((k_ipv4_verify_run_dma<U_, R_>), dim3(run_dma_blocks(d)), dim3(kBlock), 0, s, d, ip, l4, st, bad); \
-    return launched();                                                                                       \
+    return launch(k_ipv4_verify_run_dma<U_, R_>, dim3(run_dma_blocks(d)), dim3(kBlock), s, d, ip, l4, st, bad); \
   }
     MI_RUN_DMA_SHAPES(X)
 #undef X
@@ -2601,24 +2603,19 @@ int launch_verify(const Desc &d, uint32_t max_len, uint16_t *ip, uint16_t *l4, u
     const dim3 grid(run_blocks(d, pl.run_nw)), blk(64 * pl.run_nw);
 #define X(U_, NW_)                                                                                           \
   if (pl.run_u == U_ && pl.run_nw == NW_) {                                                                  \
-    VLAUNCH((k_ipv4_verify_packed<U_, 0, NW_>), grid, blk, 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);         \
-    return launched();                                                                                       \
+    return launch(k_ipv4_verify_packed<U_, 0, NW_>, grid, blk, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);      \
   }
     if (pl.occ && pl.run_nw == 2 && pl.run_u == 4) {
-      VLAUNCH((k_ipv4_verify_packed_occ<4>), grid, blk, 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-      return launched();
+      return launch(k_ipv4_verify_packed_occ<4>, grid, blk, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
     }
     if (pl.occ && pl.run_nw == 2 && pl.run_u == 8) {
-      VLAUNCH((k_ipv4_verify_packed_occ<8>), grid, blk, 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-      return launched();
+      return launch(k_ipv4_verify_packed_occ<8>, grid, blk, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
     }
     if (pl.pipe && pl.run_nw == 2 && pl.run_u == 4) {
-      VLAUNCH((k_ipv4_verify_packed<4, 0, 2, true>), grid, blk, 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-      return launched();
+      return launch(k_ipv4_verify_packed<4, 0, 2, true>, grid, blk, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
     }
     if (pl.pipe && pl.run_nw == 2 && pl.run_u == 8) {
-      VLAUNCH((k_ipv4_verify_packed<8, 0, 2, true>), grid, blk, 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-      return launched();
+      return launch(k_ipv4_verify_packed<8, 0, 2, true>, grid, blk, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
     }
     X(4, 1) X(4, 2) X(8, 1) X(8, 2)
 #undef X
@@ -2626,16 +2623,13 @@ int launch_verify(const Desc &d, uint32_t max_len, uint16_t *ip, uint16_t *l4, u
   if (pl.kind == kPlanRun) {
     const dim3 grid(run_blocks(d));
     if (pl.run_u == 4)
-      VLAUNCH((k_ipv4_verify_packed<4>), grid, dim3(kBlock), 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-    else if (pl.run_u == 16)
-      VLAUNCH((k_ipv4_verify_packed<16>), grid, dim3(kBlock), 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-    else
-      VLAUNCH((k_ipv4_verify_packed<8>), grid, dim3(kBlock), 0, s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
-    return launched();
+      return launch(k_ipv4_verify_packed<4>, grid, dim3(kBlock), s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
+    if (pl.run_u == 16)
+      return launch(k_ipv4_verify_packed<16>, grid, dim3(kBlock), s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
+    return launch(k_ipv4_verify_packed<8>, grid, dim3(kBlock), s, d, ip, l4, st, bad, SpanSeeds{}, 0u);
   }
   if (pl.kind == kPlanSlot64) {
-    VLAUNCH(k_ipv4_verify_slot64, dim3(slot64_blocks(d)), dim3(kBlock), 0, s, d, ip, l4, st, bad);
-    return launched();
+    return launch(k_ipv4_verify_slot64, dim3(slot64_blocks(d)), dim3(kBlock), s, d, ip, l4, st, bad);
   }
   if (pl.kind == kPlanShape) return launch_verify_shape(d, pl.shape, ip, l4, st, bad, s);
   for (int c = 0; c + 1 < (int)(sizeof kClassEdges / sizeof kClassEdges[0]); ++c) {
@@ -2661,15 +2655,13 @@ int launch_span(const Desc &d, Shape sh, uint32_t abs_lanes, const SpanSeeds &sd
     uint64_t blocks = ((uint64_t)d.n + 255) / 256;
     const int cap = g_tune.max_blocks > 0 ? g_tune.max_blocks : 16384;
     if (blocks > (uint64_t)cap) blocks = cap;
-    hipLaunchKernelGGL((k_ipv4_verify_packed<8, 2>), dim3(blocks ? (unsigned)blocks : 1u), dim3(kBlock), 0, s, d,
-                       out, nullptr, nullptr, nullptr, sd, abs_lanes);
-    return launched();
+    return launch(k_ipv4_verify_packed<8, 2>, dim3(blocks ? (unsigned)blocks : 1u), dim3(kBlock), s, d, out,
+                  nullptr, nullptr, nullptr, sd, abs_lanes);
   }
   const int grid = grid_for(d.n, sh.g);
 #define X(G_, U_)                                                                          \
   if (sh.g == G_ && sh.u == U_) {                                                          \
-    hipLaunchKernelGGL((k_span<G_, U_>), dim3(grid), dim3(kBlock), 0, s, d, abs_lanes, sd, out); \
-    return launched();                                                                     \
+    return launch(k_span<G_, U_>, dim3(grid), dim3(kBlock), s, d, abs_lanes, sd, out);     \
   }
   FOR_GU(X)
 #undef X
@@ -2710,19 +2702,15 @@ int launch_finalize(const Desc &d, Shape sh, hipStream_t s, uint32_t max_len) {
     uint64_t blocks = ((uint64_t)d.n + 255) / 256;
     const int cap = g_tune.max_blocks > 0 ? g_tune.max_blocks : 16384;
     if (blocks > (uint64_t)cap) blocks = cap;
-    VLAUNCH((k_ipv4_verify_packed<4, 1>), dim3(blocks ? (unsigned)blocks : 1u), dim3(kBlock), 0, s, d, nullptr,
-            nullptr, nullptr, nullptr, SpanSeeds{}, 0u);
-    return launched();
+    return launch(k_ipv4_verify_packed<4, 1>, dim3(blocks ? (unsigned)blocks : 1u), dim3(kBlock), s, d,
+                  nullptr, nullptr, nullptr, nullptr, SpanSeeds{}, 0u);
   }
   const int grid = grid_for(d.n, sh.g);
   const bool blocks = finalize_blocks_ok(d, max_len) && sh.g >= 4;
 #define X(G_, U_)                                                                          \
   if (sh.g == G_ && sh.u == U_) {                                                          \
-    if (blocks)                                                                            \
-      VLAUNCH((k_ipv4_finalize<G_, U_, true>), dim3(grid), dim3(kBlock), 0, s, d);         \
-    else                                                                                   \
-      VLAUNCH((k_ipv4_finalize<G_, U_, false>), dim3(grid), dim3(kBlock), 0, s, d);        \
-    return launched();                                                                     \
+    if (blocks) return launch(k_ipv4_finalize<G_, U_, true>, dim3(grid), dim3(kBlock), s, d); \
+    return launch(k_ipv4_finalize<G_, U_, false>, dim3(grid), dim3(kBlock), s, d);         \
   }
   FOR_GU(X)
 #undef X
@@ -2801,8 +2789,7 @@ int launch_tx(const TxDesc &t, Shape sh, hipStream_t s) {
   jnote("  status", t.status, t.n);
   if (tx_kernel_kind() == 2) {
     // one frame per wave: four per workgroup
-    hipLaunchKernelGGL((k_tx_wave<2>), dim3(grid_for(t.n, 64)), dim3(kBlock), 0, s, t);
-    return launched();
+    return launch(k_tx_wave<2>, dim3(grid_for(t.n, 64)), dim3(kBlock), s, t);
   }
   if (tx_kernel_kind() == 3 && !tx_shape_forced()) {
     // the LDS-staged gather: one wave (8 frames) per workgroup, the same total
@@ -2814,41 +2801,33 @@ int launch_tx(const TxDesc &t, Shape sh, hipStream_t s) {
     if (const char *e = getenv("MI_CKSUM_TX_LDS")) (void)sscanf(e, "%dx%d", &u, &r);
     // 16 lanes per frame (4 frames per wave, twice the waves): "2x2g16"
     if (const char *e = getenv("MI_CKSUM_TX_LDS"); e && u == 2 && r == 2 && strstr(e, "g16")) {
-      hipLaunchKernelGGL((k_tx_lds<2, 2, tx_lds_waves(2, 2), false, 16>), dim3(tx_lds_grid(t.n, (unsigned)grid_for(t.n, 8), 16)),
-                         dim3(64), 0, s, t);
-      return launched();
+      return launch(k_tx_lds<2, 2, tx_lds_waves(2, 2), false, 16>,
+                    dim3(tx_lds_grid(t.n, (unsigned)grid_for(t.n, 8), 16)), dim3(64), s, t);
     }
     // the cut cache (k_tx_lds CC): MI_CKSUM_TX_LDS = "2x2c"
     if (const char *e = getenv("MI_CKSUM_TX_LDS"); e && u == 2 && r == 2 && strchr(e, 'c')) {
-      hipLaunchKernelGGL((k_tx_lds<2, 2, tx_lds_waves(2, 2), true>), dim3(grid ? grid : 1u), dim3(64), 0, s, t);
-      return launched();
+      return launch(k_tx_lds<2, 2, tx_lds_waves(2, 2), true>, dim3(grid ? grid : 1u), dim3(64), s, t);
     }
 #define X(U_, R_)                                                                         \
   if (u == U_ && r == R_) {                                                               \
-    hipLaunchKernelGGL((k_tx_lds<U_, R_>), dim3(grid ? grid : 1u), dim3(64), 0, s, t);    \
-    return launched();                                                                    \
+    return launch(k_tx_lds<U_, R_>, dim3(grid ? grid : 1u), dim3(64), s, t);              \
   }
     X(2, 2) X(2, 3) X(2, 4) X(1, 4)
 #undef X
     // U = 1, R = 3 at 5 waves per SIMD (96 VGPRs, no scratch; 6 KiB of ring)
     if (u == 1 && r == 3) {
-      hipLaunchKernelGGL((k_tx_lds<1, 3, 5>), dim3(grid ? grid : 1u), dim3(64), 0, s, t);
-      return launched();
+      return launch(k_tx_lds<1, 3, 5>, dim3(grid ? grid : 1u), dim3(64), s, t);
     }
     return set_err(-EINVAL, "no LDS TX kernel %dx%d", u, r);
   }
   const int grid = grid_for(t.n, sh.g);
   if (sh.g == 8 && sh.u == 2) {
-    if (tx_early_loads())
-      hipLaunchKernelGGL((k_tx_copy<8, 2, true>), dim3(grid), dim3(kBlock), 0, s, t);
-    else
-      hipLaunchKernelGGL((k_tx_copy<8, 2, false>), dim3(grid), dim3(kBlock), 0, s, t);
-    return launched();
+    if (tx_early_loads()) return launch(k_tx_copy<8, 2, true>, dim3(grid), dim3(kBlock), s, t);
+    return launch(k_tx_copy<8, 2, false>, dim3(grid), dim3(kBlock), s, t);
   }
 #define X(G_, U_)                                                                  \
   if (sh.g == G_ && sh.u == U_) {                                                  \
-    hipLaunchKernelGGL((k_tx_copy<G_, U_>), dim3(grid), dim3(kBlock), 0, s, t);    \
-    return launched();                                                             \
+    return launch(k_tx_copy<G_, U_>, dim3(grid), dim3(kBlock), s, t);              \
   }
   FOR_TX_GU(X)
 #undef X
@@ -4271,8 +4250,7 @@ int mi_cksum_chain_batch(const mi_chain_batch *b, uint16_t *out, void *stream) {
   jnote("  out", out, 2ull * cd.n);
 #define X(G_, U_)                                                                              \
   if (sh.g == G_ && sh.u == U_) {                                                              \
-    hipLaunchKernelGGL((k_chain<G_, U_>), dim3(grid), dim3(kBlock), 0, st, cd, out);            \
-    return launched();                                                                         \
+    return launch(k_chain<G_, U_>, dim3(grid), dim3(kBlock), st, cd, out);                     \
   }
   FOR_GU(X)
 #undef X
@@ -4308,9 +4286,8 @@ int mi__verify_ranges(const mi_pkt_batch *b, const uint32_t *starts, uint32_t nr
   batch_activity(t_ctx.device);
   jdesc("launch verify (ranges)", nr, d, ip_sum, l4_sum, status, bad_count);
   const unsigned blocks = (nr + 1u) / 2u;
-  hipLaunchKernelGGL((k_ipv4_verify_ranges<8, 2>), dim3(blocks), dim3(128), 0, (hipStream_t)stream, d, ip_sum, l4_sum,
-                     status, bad_count, starts, nr, ends);
-  return launched();
+  return launch(k_ipv4_verify_ranges<8, 2>, dim3(blocks), dim3(128), (hipStream_t)stream, d, ip_sum, l4_sum,
+                status, bad_count, starts, nr, ends);
 }
 
 int mi_cksum_ipv4_verify_multi(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip, uint16_t *const *l4,
@@ -4385,8 +4362,7 @@ int mi_cksum_ipv4_verify_multi(const mi_pkt_batch *b, uint32_t nb, uint16_t *con
     if (!res_[dv_].load()) res_[dv_].store(resident((const void *)k_ipv4_verify_multi<G_, U_>));  \
     const uint64_t cap_ = g_tune.max_blocks > 0 ? (uint64_t)g_tune.max_blocks : res_[dv_].load(); \
     if (blocks > cap_) blocks = cap_;                                                             \
-    VLAUNCH((k_ipv4_verify_multi<G_, U_>), dim3((unsigned)blocks), dim3(kBlock), 0, s, a);       \
-    return launched();                                                                            \
+    return launch(k_ipv4_verify_multi<G_, U_>, dim3((unsigned)blocks), dim3(kBlock), s, a);       \
   }
   FOR_GU(X)
 #undef X
@@ -5016,14 +4992,10 @@ int mi_cksum_synth_ipv4(const mi_pkt_batch *b, uint64_t seed, void *stream) {
   if (fill) {
     uint64_t blocks = (fill / 16 + kBlock - 1) / kBlock;
     if (blocks > 8192) blocks = 8192;
-    hipLaunchKernelGGL(k_fill, dim3((unsigned)blocks), dim3(kBlock), 0, st, (uint8_t *)b->base, fill, seed);
-    HIP_TRY(hipGetLastError());
+    if ((rc = launch(k_fill, dim3((unsigned)blocks), dim3(kBlock), st, (uint8_t *)b->base, fill, seed))) return rc;
   }
-  if (d.n) {
-    hipLaunchKernelGGL(k_synth_hdr, dim3((d.n + kBlock - 1) / kBlock), dim3(kBlock), 0, st, d);
-    HIP_TRY(hipGetLastError());
-  }
-  return 0;
+  if (!d.n) return 0;
+  return launch(k_synth_hdr, dim3((d.n + kBlock - 1) / kBlock), dim3(kBlock), st, d);
 }
 
 // Ranges registered through mi_cksum_host_register: the zero-copy path reads
@@ -5788,10 +5760,10 @@ int mi__scalar_fold(size_t off, uint32_t len, uint32_t lanes, int pseudo, uint32
   } else {
     // (the HIP fallback, MI_CKSUM_HOST_AQL=0: its stream only now, place_*)
     if (!c.sstream) HIP_TRY(hipStreamCreateWithFlags(&c.sstream, hipStreamNonBlocking));
-    hipLaunchKernelGGL(mi_aql_scalar, dim3(1), dim3(kScalarThreads), 0, c.sstream, (const uint8_t *)c.stage_dev,
-                       (uint32_t)c.stage_cap, (uint32_t)off, len, lanes == MI_SPAN_ABS ? 1u : 0u, pseudo, src, dst,
-                       (uint32_t)proto, plen, tag | (trace ? 0x80000000u : 0u), c.sout_dev);
-    HIP_TRY(hipGetLastError());
+    if ((rc = launch(mi_aql_scalar, dim3(1), dim3(kScalarThreads), c.sstream, (const uint8_t *)c.stage_dev,
+                     (uint32_t)c.stage_cap, (uint32_t)off, len, lanes == MI_SPAN_ABS ? 1u : 0u, pseudo, src, dst,
+                     (uint32_t)proto, plen, tag | (trace ? 0x80000000u : 0u), c.sout_dev)))
+      return rc;
   }
   volatile uint32_t *slot = c.sout;
   uint32_t v = 0;
@@ -5904,9 +5876,7 @@ int mi__spin(uint32_t us, int via) {
   const uint64_t ticks = (uint64_t)us * 100u;
   if (via == 0) {
     if (!t_ctx.sstream) HIP_TRY(hipStreamCreateWithFlags(&t_ctx.sstream, hipStreamNonBlocking));
-    hipLaunchKernelGGL(mi_aql_spin, dim3(1), dim3(64), 0, t_ctx.sstream, ticks);
-    HIP_TRY(hipGetLastError());
-    return 0;
+    return launch(mi_aql_spin, dim3(1), dim3(64), t_ctx.sstream, ticks);
   }
   AqlOne &o = t_aql1;
   if ((rc = aql_one_open(o))) return rc;

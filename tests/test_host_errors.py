@@ -1,0 +1,88 @@
+"""What the library's host code does when a HIP call fails: over a runtime of
+host memory (tests/hip_stub.cpp), on the CPU."""
+import pytest
+
+import stubbed
+
+import libunsod_amd as mi
+
+pytestmark = pytest.mark.skipif(mi.device_count() > 0, reason="the stub runtime stands in for a missing GPU")
+
+
+@pytest.fixture(scope="module")
+def so(tmp_path_factory):
+    return stubbed.build(tmp_path_factory.mktemp("hip_stub"))
+
+
+# every entry point that launches: (name, the call)
+LAUNCHES = r'''
+n = 64
+b = batch(n)
+o16, o8, o32 = np.zeros(2 * n, np.uint16), np.zeros(n, np.uint8), np.zeros(2 * n, np.uint32)
+p16, p8, p32 = o16.ctypes.data, o8.ctypes.data, o32.ctypes.data
+seg_off, seg_len = (np.arange(n) * 2176).astype(np.uint64), np.full(n, 1500, np.int32)
+pkt_seg, clen, skip = np.arange(n + 1, dtype=np.uint32), np.full(n, 1500, np.int32), np.zeros(n, np.int32)
+cb = _lib.ChainBatchC(b.base, b.bytes, seg_off.ctypes.data, seg_len.ctypes.data, pkt_seg.ctypes.data, n, 0,
+                      clen.ctypes.data, skip.ctypes.data, None, None, None, 1500, n)
+tb = tx_batch(8)
+one = (C.c_void_p * 1)
+st1 = one(p8)
+rep, trep = C.c_void_p(), C.c_void_p()
+assert lib.mi_cksum_repeat_create(C.byref(b), 1, None, None, st1, 1, C.byref(rep)) == 0, err()
+assert lib.mi_cksum_tx_repeat_create(C.byref(tb), 1, st1, 1, C.byref(trep)) == 0, err()
+us = C.c_float()
+lens = np.full(n, 1500, np.uint32)
+classes = batch(n, lens=lens)
+dense = batch(n, L=46, stride=64)
+tight = batch(n, L=100, stride=128)
+entries = {
+    "verify": lambda: lib.mi_cksum_ipv4_verify(C.byref(b), p16, None, p8, None, None),
+    "verify, length classes": lambda: lib.mi_cksum_ipv4_verify(C.byref(classes), p16, None, p8, None, None),
+    "verify, 64-byte slots": lambda: lib.mi_cksum_ipv4_verify(C.byref(dense), p16, None, p8, None, None),
+    "verify, flat run": lambda: lib.mi_cksum_ipv4_verify(C.byref(tight), p16, None, p8, None, None),
+    "verify_multi": lambda: lib.mi_cksum_ipv4_verify_multi(C.byref(b), 1, None, None, st1, None, None),
+    "rx_offload": lambda: lib.mi_cksum_rx_offload(C.byref(b), p32, None, None, None),
+    "span": lambda: lib.mi_cksum_span_batch(C.byref(b), 0, None, p16, None),
+    "chain": lambda: lib.mi_cksum_chain_batch(C.byref(cb), p16, None),
+    "finalize": lambda: lib.mi_cksum_ipv4_finalize(C.byref(b), None),
+    "finalize, flat run": lambda: lib.mi_cksum_ipv4_finalize(C.byref(tight), None),
+    "synth": lambda: lib.mi_cksum_synth_ipv4(C.byref(b), 1, None),
+    "tx_copy": lambda: lib.mi_cksum_tx_copy(C.byref(tb), p8, None),
+    "tx_copy_host": lambda: lib.mi_cksum_tx_copy_host(C.byref(tb), p8, 0),
+    "verify_host": lambda: lib.mi_cksum_ipv4_verify_host(C.byref(b), p16, None, p8, None),
+    "verify_repeat": lambda: lib.mi_cksum_ipv4_verify_repeat(C.byref(b), 1, None, None, st1, 3, 2, 0, None, None),
+    "repeat_run": lambda: lib.mi_cksum_repeat_run(rep, 3, 0, None),
+    "repeat_run, timed": lambda: lib.mi_cksum_repeat_run(rep, 3, 1, C.byref(us)),
+    "tx repeat_run": lambda: lib.mi_cksum_repeat_run(trep, 3, 0, None),
+}
+for name, call in entries.items():  # once each: contexts, staging and the first-use queries are set up
+    assert call() == 0, (name, err())
+stub.stub_set_last(0)
+'''
+
+
+def test_an_earlier_error_is_not_the_launchs(so):
+    """An error that some other call of the thread left behind is not reported
+    by the next launch, whose kernel was enqueued, and stays there for the code
+    that left it (a later failing call overwrites it: chain and TX calls ask the
+    runtime for the extent of tables it does not know)."""
+    stubbed.run(so, LAUNCHES + r'''
+for name, call in entries.items():
+    stub.stub_set_last(INVALID)
+    before, errors = calls("hipLaunchKernel") + calls("hipExtLaunchKernel"), stub.stub_errors()
+    assert call() == 0, (name, err())
+    assert calls("hipLaunchKernel") + calls("hipExtLaunchKernel") > before, name
+    assert stub.stub_last() == (INVALID if stub.stub_errors() == errors else 0), name
+''')
+
+
+def test_a_failed_launch_is_reported(so):
+    """A launch that fails is: -EIO, with the launch named, from every entry point."""
+    stubbed.run(so, LAUNCHES + r'''
+for name, call in entries.items():
+    fn = "hipExtLaunchKernel" if name == "repeat_run, timed" else "hipLaunchKernel"
+    fail(fn, err=700)
+    assert call() == EIO, name
+    assert "stub error 700" in err() and "aunch" in err(), (name, err())
+    assert call() == 0, (name, err())
+''')
