@@ -1900,9 +1900,17 @@ int set_err(int code, const char *fmt, ...) {
   return code;
 }
 
+// e, taken out of the thread's last error (hipGetLastError) where it is one: a
+// failure that the library reports through its own return code, or recovers
+// from, must not be found there by a later check, the library's or the caller's.
+hipError_t cleared(hipError_t e) {
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
+}
+
 #define HIP_TRY(expr)                                                                   \
   do {                                                                                  \
-    hipError_t e_ = (expr);                                                             \
+    hipError_t e_ = cleared(expr);                                                      \
     if (e_ != hipSuccess)                                                               \
       return set_err(-EIO, "%s: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__,  \
                      __LINE__);                                                        \
@@ -1946,31 +1954,28 @@ void jnote(const char *what, const void *p = nullptr, uint64_t bytes = 0, uint32
 uint64_t alloc_bytes(const void *p) {
   hipDeviceptr_t base = nullptr;
   size_t size = 0;
-  if (!p || hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p) != hipSuccess) {
-    (void)hipGetLastError();
-    return 0;
-  }
+  if (!p || cleared(hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p)) != hipSuccess) return 0;
   return size;
 }
 template <typename T>
 hipError_t jmalloc(T **p, size_t n) {
-  const hipError_t e = hipMalloc((void **)p, n);
+  const hipError_t e = cleared(hipMalloc((void **)p, n));
   if (e == hipSuccess) jnote("alloc device", *p, n);
   return e;
 }
 template <typename T>
 hipError_t jhostmalloc(T **p, size_t n, unsigned flags) {
-  const hipError_t e = hipHostMalloc((void **)p, n, flags);
+  const hipError_t e = cleared(hipHostMalloc((void **)p, n, flags));
   if (e == hipSuccess) jnote("alloc host", *p, n);
   return e;
 }
 hipError_t jfree(void *p) {
   if (p) jnote("free device", p, alloc_bytes(p));
-  return hipFree(p);
+  return cleared(hipFree(p));
 }
 hipError_t jhostfree(void *p) {
   if (p) jnote("free host", p, alloc_bytes(p));
-  return hipHostFree(p);
+  return cleared(hipHostFree(p));
 }
 hsa_status_t fault_event(const hsa_amd_event_t *ev, void *) {
   if (!ev || ev->event_type != HSA_AMD_GPU_MEMORY_FAULT_EVENT) return HSA_STATUS_SUCCESS;
@@ -2097,11 +2102,11 @@ int check_device(int dev) {
 // Free everything a context holds (on its own device; `back` is made current
 // again afterwards).  Errors are ignored: this is cleanup.
 void ctx_release(ThreadCtx &c, int back) {
-  if (hipSetDevice(c.device) != hipSuccess) return;
+  if (cleared(hipSetDevice(c.device)) != hipSuccess) return;
   auto stream = [](hipStream_t &s) {
     if (s) {
-      (void)hipStreamSynchronize(s);
-      (void)hipStreamDestroy(s);
+      (void)cleared(hipStreamSynchronize(s));
+      (void)cleared(hipStreamDestroy(s));
       s = nullptr;
     }
   };
@@ -2133,17 +2138,17 @@ void ctx_release(ThreadCtx &c, int back) {
   dfree(c.rdeal);
   for (int q = 0; q < ThreadCtx::kMaxRep; ++q) {
     stream(c.rstream[q]);
-    if (c.rjoin[q]) (void)hipEventDestroy(c.rjoin[q]);
+    if (c.rjoin[q]) (void)cleared(hipEventDestroy(c.rjoin[q]));
   }
   for (auto &g : c.rgraph)
-    if (g.exec) (void)hipGraphExecDestroy(g.exec);
-  if (c.rgate) (void)hipEventDestroy(c.rgate);
-  if (c.rfork) (void)hipEventDestroy(c.rfork);
-  for (uint32_t e = 0; e < c.nev; ++e) (void)hipEventDestroy(c.ev[e]);
+    if (g.exec) (void)cleared(hipGraphExecDestroy(g.exec));
+  if (c.rgate) (void)cleared(hipEventDestroy(c.rgate));
+  if (c.rfork) (void)cleared(hipEventDestroy(c.rfork));
+  for (uint32_t e = 0; e < c.nev; ++e) (void)cleared(hipEventDestroy(c.ev[e]));
   free(c.ev);
   c.ev = nullptr;
   c.nev = 0;
-  (void)hipSetDevice(back);
+  (void)cleared(hipSetDevice(back));
 }
 
 void thread_exit_register();
@@ -2152,7 +2157,7 @@ bool retire_dropins();
 // Make sure the calling thread has a context on its current HIP device.
 int ensure_ctx() {
   int dev = -1;
-  hipError_t e = hipGetDevice(&dev);
+  hipError_t e = cleared(hipGetDevice(&dev));
   if (e != hipSuccess) return set_err(-ENODEV, "no HIP device: %s", hipGetErrorString(e));
   if (t_ctx.device == dev) return 0;
   int rc = check_device(dev);
@@ -2246,10 +2251,7 @@ uint64_t alloc_extent(const void *p, uint64_t want) {
   if (!p) return 0;
   hipDeviceptr_t base = nullptr;
   size_t size = 0;
-  if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p) != hipSuccess || !base) {
-    (void)hipGetLastError();  // (not an error of the caller's: clear it)
-    return want;
-  }
+  if (cleared(hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p)) != hipSuccess || !base) return want;
   const uint64_t end = (uint64_t)(uintptr_t)base + size, a = (uint64_t)(uintptr_t)p;
   return a < end ? std::min<uint64_t>(want, end - a) : 0;
 }
@@ -2327,13 +2329,13 @@ int launch(void (*k)(P...), dim3 grid, dim3 block, hipStream_t s, A... a) {
   std::tuple<P...> p(a...);
   const LaunchEv ev = t_lev;
   t_lev = LaunchEv();
-  const hipError_t e = std::apply(
+  const hipError_t e = cleared(std::apply(
       [&](auto &...v) {
         void *args[] = {(void *)&v...};
         return ev.start || ev.stop ? hipExtLaunchKernel((const void *)k, grid, block, args, 0, s, ev.start, ev.stop, 0)
                                    : hipLaunchKernel((const void *)k, grid, block, args, 0, s);
       },
-      p);
+      p));
   if (e != hipSuccess) return set_err(-EIO, "kernel launch: %s", hipGetErrorString(e));
   return 0;
 }
@@ -2543,10 +2545,9 @@ unsigned resident_blocks(const void *fn) {
     if (e.first.first == fn && e.first.second == dev) return e.second;
   int per_cu = 0, cus = 0;
   unsigned r = 0;
-  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, kBlock, 0) == hipSuccess && per_cu > 0 &&
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0)
+  if (cleared(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, kBlock, 0)) == hipSuccess && per_cu > 0 &&
+      cleared(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev)) == hipSuccess && cus > 0)
     r = (unsigned)(per_cu * cus);
-  (void)hipGetLastError();
   cache.push_back({{fn, dev}, r});
   return r;
 }
@@ -3132,10 +3133,11 @@ int aql_device(int dev, AqlDevice **out) {
     // HIP may load a code object lazily: querying the kernels loads it
     for (int i = 0; i < kAqlKernels && !a.rc; ++i) {
       hipFuncAttributes fa;
-      if (hipFuncGetAttributes(&fa, kAqlFuncs[i]) != hipSuccess) fail(-EIO, "hipFuncGetAttributes(%s)", kAqlNames[i]);
+      if (cleared(hipFuncGetAttributes(&fa, kAqlFuncs[i])) != hipSuccess)
+        fail(-EIO, "hipFuncGetAttributes(%s)", kAqlNames[i]);
     }
     hipDeviceProp_t prop;
-    if (!a.rc && hipGetDeviceProperties(&prop, dev) != hipSuccess) fail(-EIO, "hipGetDeviceProperties");
+    if (!a.rc && cleared(hipGetDeviceProperties(&prop, dev)) != hipSuccess) fail(-EIO, "hipGetDeviceProperties");
     if (!a.rc && hsa_init() != HSA_STATUS_SUCCESS) fail(-EIO, "hsa_init");
     AqlAgentFind af{(uint32_t)((prop.pciBusID << 8) | (prop.pciDeviceID << 3)), (uint32_t)prop.pciDomainID, {}, false};
     if (!a.rc) {
@@ -3397,7 +3399,7 @@ int aql_create(int device, const Desc *d, const uint32_t *max_len, uint16_t *con
   // carries its queue's counter set (passes of one queue never overlap)
   if (any_deal) {
     hipError_t e = jmalloc(&a->deal, (size_t)kDealSetBytes * nq);
-    if (e == hipSuccess) e = hipMemset(a->deal, 0, (size_t)kDealSetBytes * nq);
+    if (e == hipSuccess) e = cleared(hipMemset(a->deal, 0, (size_t)kDealSetBytes * nq));
     if (e != hipSuccess) {
       aql_free(a);
       return set_err(-ENOMEM, "AQL engine: counters: %s", hipGetErrorString(e));
@@ -3429,7 +3431,7 @@ int aql_create(int device, const Desc *d, const uint32_t *max_len, uint16_t *con
     jdesc("  aql batch", (uint32_t)ids[j], d[j], ip ? ip[j] : nullptr, l4 ? l4[j] : nullptr, st ? st[j] : nullptr);
   }
   if (a->deal) jnote("  aql deal counters", a->deal, (uint64_t)kDealSetBytes * nq);
-  e = hipMemcpy(a->kargs, host.data(), host.size(), hipMemcpyHostToDevice);
+  e = cleared(hipMemcpy(a->kargs, host.data(), host.size(), hipMemcpyHostToDevice));
   if (e != hipSuccess) {
     aql_free(a);
     return set_err(-EIO, "AQL engine: kernel arguments: %s", hipGetErrorString(e));
@@ -3498,7 +3500,7 @@ int aql_create_tx(int device, const TxDesc *t, uint32_t nb, uint32_t nqueues, Aq
     jnote("  aql tx src", t[j].src, t[j].src_bytes, t[j].n);
     jnote("  aql tx dst", t[j].dst, t[j].dst_bytes);
   }
-  e = hipMemcpy(a->kargs, host.data(), host.size(), hipMemcpyHostToDevice);
+  e = cleared(hipMemcpy(a->kargs, host.data(), host.size(), hipMemcpyHostToDevice));
   if (e != hipSuccess) {
     aql_free(a);
     return set_err(-EIO, "AQL engine: kernel arguments: %s", hipGetErrorString(e));
@@ -3725,7 +3727,7 @@ int slab_alloc(AqlDevice *a) {
   }
   if (!a->slab) {
     if (jhostmalloc((void **)&a->slab, kSlabBytes, hipHostMallocMapped | hipHostMallocCoherent) != hipSuccess ||
-        hipHostGetDevicePointer((void **)&a->slab_dev, a->slab, 0) != hipSuccess) {
+        cleared(hipHostGetDevicePointer((void **)&a->slab_dev, a->slab, 0)) != hipSuccess) {
       a->slab = a->slab_dev = nullptr;
       return set_err(-ENOMEM, "drop-in service: mailbox slab");
     }
@@ -3753,7 +3755,7 @@ int dq_open(AqlDevice *a) {
     rc = set_err(-ENOMEM, "drop-in service: kernel-argument block");
   uint32_t *h = nullptr;
   if (!rc && (jhostmalloc((void **)&h, 64, hipHostMallocMapped | hipHostMallocCoherent) != hipSuccess ||
-              hipHostGetDevicePointer((void **)&a->svc_host_dev, (void *)h, 0) != hipSuccess))
+              cleared(hipHostGetDevicePointer((void **)&a->svc_host_dev, (void *)h, 0)) != hipSuccess))
     rc = set_err(-ENOMEM, "drop-in service: exit word");
   if (!rc) rc = slab_alloc(a);
   if (rc) {
@@ -4161,7 +4163,7 @@ const char *mi_cksum_strerror(void) { return t_err; }
 
 int mi_cksum_device_count(void) {
   int n = 0;
-  if (hipGetDeviceCount(&n) != hipSuccess) return 0;
+  if (cleared(hipGetDeviceCount(&n)) != hipSuccess) return 0;
   return n;
 }
 
@@ -4350,8 +4352,8 @@ int mi_cksum_ipv4_verify_multi(const mi_pkt_batch *b, uint32_t nb, uint16_t *con
   auto resident = [&](const void *fn) -> uint64_t {
     int per_cu = 0, dev = t_ctx.device;
     hipDeviceProp_t prop;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, kBlock, 0) != hipSuccess || per_cu <= 0 ||
-        hipGetDeviceProperties(&prop, dev) != hipSuccess)
+    if (cleared(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, kBlock, 0)) != hipSuccess || per_cu <= 0 ||
+        cleared(hipGetDeviceProperties(&prop, dev)) != hipSuccess)
       return 2048;
     return (uint64_t)per_cu * (uint64_t)prop.multiProcessorCount;
   };
@@ -4446,7 +4448,7 @@ int mi_cksum_ipv4_verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *co
     if (!c.rstream[q]) HIP_TRY(hipStreamCreateWithFlags(&c.rstream[q], hipStreamNonBlocking));
   const uint32_t need_ev = timing == MI_TIME_PER_PASS ? 2 * steps : 2 + nstreams;
   if (c.nev < need_ev) {
-    for (uint32_t e = 0; e < c.nev; ++e) (void)hipEventDestroy(c.ev[e]);
+    for (uint32_t e = 0; e < c.nev; ++e) (void)cleared(hipEventDestroy(c.ev[e]));
     free(c.ev);
     c.nev = 0;
     c.ev = (hipEvent_t *)calloc(need_ev, sizeof(hipEvent_t));
@@ -4509,15 +4511,15 @@ int mi_cksum_ipv4_verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *co
       hipGraph_t g = nullptr;
       HIP_TRY(hipStreamEndCapture(c.rstream[0], &g));
       if (rc) {
-        (void)hipGraphDestroy(g);
+        (void)cleared(hipGraphDestroy(g));
         return rc;
       }
       gr = &c.rgraph[c.rgraph_next];
       c.rgraph_next = (c.rgraph_next + 1) % ThreadCtx::kGraphs;
-      if (gr->exec) (void)hipGraphExecDestroy(gr->exec);
+      if (gr->exec) (void)cleared(hipGraphExecDestroy(gr->exec));
       gr->exec = nullptr;
       HIP_TRY(hipGraphInstantiate(&gr->exec, g, nullptr, nullptr, 0));
-      (void)hipGraphDestroy(g);
+      (void)cleared(hipGraphDestroy(g));
       gr->key = key;
       gr->steps = steps;
       gr->nstreams = nstreams;
@@ -4602,12 +4604,12 @@ namespace {
 void repeat_free(mi_repeat *r) {
   if (!r) return;
   for (uint32_t q = 0; q < ThreadCtx::kMaxRep; ++q) {
-    if (r->s[q]) (void)hipStreamSynchronize(r->s[q]);
-    if (r->ev_end[q]) (void)hipEventDestroy(r->ev_end[q]);
-    if (r->ev_done[q]) (void)hipEventDestroy(r->ev_done[q]);
-    if (r->s[q]) (void)hipStreamDestroy(r->s[q]);
+    if (r->s[q]) (void)cleared(hipStreamSynchronize(r->s[q]));
+    if (r->ev_end[q]) (void)cleared(hipEventDestroy(r->ev_end[q]));
+    if (r->ev_done[q]) (void)cleared(hipEventDestroy(r->ev_done[q]));
+    if (r->s[q]) (void)cleared(hipStreamDestroy(r->s[q]));
   }
-  if (r->ev0) (void)hipEventDestroy(r->ev0);
+  if (r->ev0) (void)cleared(hipEventDestroy(r->ev0));
   if (r->flag) (void)jhostfree(r->flag);
   if (r->deal) (void)jfree(r->deal);
   if (r->aql) {
@@ -4697,18 +4699,18 @@ int repeat_open(mi_repeat *r, uint32_t nb, uint32_t nstreams) {
   r->nstreams = nstreams;
   hipError_t e = hipSuccess;
   for (uint32_t q = 0; q < nstreams && e == hipSuccess; ++q) {
-    e = hipStreamCreateWithFlags(&r->s[q], hipStreamNonBlocking);
-    if (e == hipSuccess) e = hipEventCreate(&r->ev_end[q]);
-    if (e == hipSuccess) e = hipEventCreateWithFlags(&r->ev_done[q], hipEventDisableTiming);
+    e = cleared(hipStreamCreateWithFlags(&r->s[q], hipStreamNonBlocking));
+    if (e == hipSuccess) e = cleared(hipEventCreate(&r->ev_end[q]));
+    if (e == hipSuccess) e = cleared(hipEventCreateWithFlags(&r->ev_done[q], hipEventDisableTiming));
   }
-  if (e == hipSuccess) e = hipEventCreate(&r->ev0);
+  if (e == hipSuccess) e = cleared(hipEventCreate(&r->ev0));
   if (e == hipSuccess && deal_on()) {
     e = jmalloc(&r->deal, (size_t)kDealSetBytes * nstreams);
-    if (e == hipSuccess) e = hipMemset(r->deal, 0, (size_t)kDealSetBytes * nstreams);
+    if (e == hipSuccess) e = cleared(hipMemset(r->deal, 0, (size_t)kDealSetBytes * nstreams));
   }
   if (e == hipSuccess && repeat_wait_mode() == kWaitFlag) {
     e = jhostmalloc((void **)&r->flag, 64 * sizeof(uint32_t), hipHostMallocMapped | hipHostMallocCoherent);
-    if (e == hipSuccess) e = hipHostGetDevicePointer((void **)&r->flag_dev, r->flag, 0);
+    if (e == hipSuccess) e = cleared(hipHostGetDevicePointer((void **)&r->flag_dev, r->flag, 0));
     if (e == hipSuccess) memset(r->flag, 0, 64 * sizeof(uint32_t));
   }
   if (e != hipSuccess) {
@@ -4800,7 +4802,7 @@ int mi_cksum_repeat_run(mi_repeat *r, uint32_t steps, uint32_t flags, float *spa
   for (uint32_t q = 0; q < ns; ++q) {
     if (wm == kWaitSpin) {
       hipError_t e;
-      while ((e = hipEventQuery(fin[q])) == hipErrorNotReady) {
+      while ((e = cleared(hipEventQuery(fin[q]))) == hipErrorNotReady) {
       }
       if (e != hipSuccess) return set_err(-EIO, "hipEventQuery: %s", hipGetErrorString(e));
     } else if (wm == kWaitEvent) {
@@ -5062,8 +5064,8 @@ int mi_cksum_host_register(void *p, uint64_t bytes) {
   jnote("host register pages", (const void *)lo, hi - lo);
   dbg_mem("host-register", p, bytes);
   void *dev = nullptr;
-  if (hipHostGetDevicePointer(&dev, p, 0) != hipSuccess || !dev) {
-    (void)hipHostUnregister(p);
+  if (cleared(hipHostGetDevicePointer(&dev, p, 0)) != hipSuccess || !dev) {
+    (void)cleared(hipHostUnregister(p));
     return set_err(-EIO, "mi_cksum_host_register: no device address for the range");
   }
   g_reg.push_back({lo, hi, (uintptr_t)p, (uintptr_t)dev});
@@ -5665,7 +5667,7 @@ uint8_t *mi__scalar_staging(size_t need) {
     // (every drop-in kernel has read the buffer before storing its result, so
     // once a call has returned nothing reads it -- unless a call failed
     // without its result: then the old buffer is leaked, not freed)
-    if (c.sstream && hipStreamSynchronize(c.sstream) != hipSuccess) {
+    if (c.sstream && cleared(hipStreamSynchronize(c.sstream)) != hipSuccess) {
       set_err(-EIO, "scalar staging: stream");
       return nullptr;
     }
@@ -5678,7 +5680,7 @@ uint8_t *mi__scalar_staging(size_t need) {
     size_t cap = 1;
     while (cap < need) cap <<= 1;
     hipError_t e = jhostmalloc((void **)&c.stage, cap, hipHostMallocMapped);
-    if (e == hipSuccess) e = hipHostGetDevicePointer((void **)&c.stage_dev, c.stage, 0);
+    if (e == hipSuccess) e = cleared(hipHostGetDevicePointer((void **)&c.stage_dev, c.stage, 0));
     if (e != hipSuccess) {
       set_err(-ENOMEM, "jhostmalloc(%zu): %s", cap, hipGetErrorString(e));
       return nullptr;
@@ -5784,7 +5786,7 @@ int mi__scalar_fold(size_t off, uint32_t len, uint32_t lanes, int pseudo, uint32
             return set_err(-EIO, "scalar fold: queue error 0x%x", o.dev->dq_err.load());
           }
         } else {
-          const hipError_t e = hipStreamQuery(c.sstream);
+          const hipError_t e = cleared(hipStreamQuery(c.sstream));
           if (e != hipSuccess && e != hipErrorNotReady) return set_err(-EIO, "scalar fold: %s", hipGetErrorString(e));
           retired = e == hipSuccess;
         }

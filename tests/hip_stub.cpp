@@ -83,6 +83,21 @@ void stub_fail(const char *name, int nth, int err) {
 }
 void stub_set_last(int err) { t_last = (hipError_t)err; }
 int stub_last(void) { return (int)t_last; }
+// Every function called since the last stub_reset, as "name count" lines.
+const char *stub_counts(void) {
+  static thread_local std::string out;
+  std::lock_guard<std::mutex> lk(g_mu);
+  out.clear();
+  for (auto &c : g_calls) out += c.first + " " + std::to_string(c.second) + "\n";
+  return out.c_str();
+}
+// No counts, no injected failures, no last error.
+void stub_reset(void) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  g_calls.clear();
+  g_fail.clear();
+  t_last = hipSuccess;
+}
 int stub_calls(const char *name) {
   std::lock_guard<std::mutex> lk(g_mu);
   return g_calls[name];

@@ -86,3 +86,134 @@ for name, call in entries.items():
     assert "stub error 700" in err() and "aunch" in err(), (name, err())
     assert call() == 0, (name, err())
 ''')
+
+
+# every entry point that talks to the runtime, each on a thread of its own
+# (thread contexts start empty: the first call allocates), once for every
+# runtime call it makes with that call failing
+SWEEP = r'''
+import threading
+
+n = 64
+o16, o8, o32 = np.zeros(2 * n, np.uint16), np.zeros(n, np.uint8), np.zeros(2 * n, np.uint32)
+p16, p8, p32 = o16.ctypes.data, o8.ctypes.data, o32.ctypes.data
+st1 = (C.c_void_p * 1)(p8)
+lens = np.full(n, 1500, np.uint32)
+seg_off, seg_len = (np.arange(n) * 2176).astype(np.uint64), np.full(n, 1500, np.int32)
+pkt_seg, skip = np.arange(n + 1, dtype=np.uint32), np.zeros(n, np.int32)
+b, big, mixed, tb = batch(n), batch(4 * n, stride=4096), batch(n, lens=lens), tx_batch(8)
+cb = _lib.ChainBatchC(b.base, b.bytes, seg_off.ctypes.data, seg_len.ctypes.data, pkt_seg.ctypes.data, n, 0,
+                      seg_len.ctypes.data, skip.ctypes.data, None, None, None, 1500, n)
+B = C.byref(b)
+for f in ("mi__scalar_staging",):
+    getattr(lib, f).restype, getattr(lib, f).argtypes = C.c_void_p, [C.c_size_t]
+
+
+def created(tx=False):
+    h = C.c_void_p()
+    rc = (lib.mi_cksum_tx_repeat_create(C.byref(tb), 1, st1, 2, C.byref(h)) if tx else
+          lib.mi_cksum_repeat_create(B, 1, None, None, st1, 2, C.byref(h)))
+    assert (rc == 0) == bool(h), "a handle with an error"
+    return rc, h
+
+
+def whole(tx=False):  # a handle's life
+    rc, h = created(tx)
+    if rc == 0:
+        rc = lib.mi_cksum_repeat_run(h, 3, 0, None) or lib.mi_cksum_repeat_run(h, 3, 1 | 0x200, C.byref(C.c_float()))
+        lib.mi_cksum_repeat_destroy(h)
+    return rc
+
+
+def registered(call):
+    rc = lib.mi_cksum_host_register(b.base, b.bytes)
+    if rc == 0:
+        rc = call()
+        r2 = lib.mi_cksum_host_unregister(b.base)
+        rc = rc or r2
+    return rc
+
+
+us8 = (C.c_float * 8)()
+us = C.cast(us8, C.POINTER(C.c_float))
+chunked = lambda **k: lib.mi_cksum_ipv4_verify_host(C.byref(k.get("b", b)), p16, p16 + 2 * n, p8, C.byref(C.c_uint32()))
+entries = {
+    "init": lambda: lib.mi_cksum_init(0),
+    "set_busy_wait": lambda: lib.mi_cksum_set_busy_wait(1),
+    "verify": lambda: lib.mi_cksum_ipv4_verify(B, p16, None, p8, None, None),
+    "verify_multi": lambda: lib.mi_cksum_ipv4_verify_multi(B, 1, None, None, st1, None, None),
+    "chain": lambda: lib.mi_cksum_chain_batch(C.byref(cb), p16, None),
+    "finalize": lambda: lib.mi_cksum_ipv4_finalize(B, None),
+    "synth": lambda: lib.mi_cksum_synth_ipv4(B, 1, None),
+    "tx_copy": lambda: lib.mi_cksum_tx_copy(C.byref(tb), p8, None),
+    "tx_copy_host": lambda: lib.mi_cksum_tx_copy_host(C.byref(tb), p8, 0),
+    "verify_host": chunked,
+    "verify_host, lengths": lambda: chunked(b=mixed),
+    "rx_offload_host": lambda: lib.mi_cksum_rx_offload_host(B, p32, p32 + 4 * n, C.byref(C.c_uint32())),
+    "verify_host, registered": lambda: registered(chunked),
+    "verify_repeat": lambda: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, 2, 1, None, us),
+    "verify_repeat, per pass": lambda: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, 2, 2, us, None),
+    "repeat handle": whole,
+    "tx repeat handle": lambda: whole(True),
+    "drop-in staging": lambda: 0 if lib.mi__scalar_staging(100) else -1,
+}
+
+
+def in_thread(f):
+    out = []
+
+    def go():
+        try:
+            out.append(f())
+        except BaseException as e:
+            out.append(e)
+    t = threading.Thread(target=go)
+    t.start()
+    t.join()
+    if isinstance(out[0], BaseException):
+        raise out[0]
+    return out[0]
+
+
+def counts_of(call):
+    def probe():
+        stub.stub_reset()
+        rc = call()
+        return rc, dict((k, int(v)) for k, v in (ln.split() for ln in stub.stub_counts().decode().splitlines()))
+    return in_thread(probe)
+
+
+stub.stub_counts.restype = C.c_char_p
+# HIP launches alone, and MI_CKSUM_HOST_CHUNK makes host batches several chunks
+assert os.environ["MI_CKSUM_HOST_CHUNK"] == "20000"
+in_thread(lambda: [f() for f in entries.values()])  # per-process first-use queries
+
+
+def sweep(check):
+    done = 0
+    for name, call in entries.items():
+        rc, counts = counts_of(call)
+        assert rc == 0, (name, rc, err())
+        for fn, k in counts.items():
+            for nth in range(1, k + 1):
+                def one():
+                    stub.stub_reset()
+                    fail(fn, nth, NOMEM)
+                    check((name, fn, nth), call, call())
+                    stub.stub_reset()
+                in_thread(one)
+                done += 1
+    return done
+'''
+
+
+def test_no_failure_leaves_the_last_error(so):
+    """Whatever runtime call fails, the thread's last error is clear when the
+    library returns: the failure is in its return code, or was recovered from."""
+    stubbed.run(so, SWEEP + r'''
+def check(where, call, rc):
+    assert stub.stub_last() == 0, (where, rc, stub.stub_last())
+
+
+assert sweep(check) > 200
+''', MI_CKSUM_HOST_CHUNK="20000")
