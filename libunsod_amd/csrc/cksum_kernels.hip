@@ -2062,6 +2062,8 @@ struct ThreadCtx {
   // staged TX host path: source blob, slot region, descriptors (device)
   uint8_t *tx_src = nullptr, *tx_dst = nullptr, *tx_desc = nullptr;
   size_t tx_src_cap = 0, tx_dst_cap = 0, tx_desc_cap = 0;
+  uint8_t *tx_hdesc = nullptr;  // the descriptors on the host (malloc): an async copy reads them
+  size_t tx_hdesc_cap = 0;
   // repeat-launch streams and timing events
   static constexpr int kMaxRep = 8;
   hipStream_t rstream[kMaxRep] = {};
@@ -2099,6 +2101,40 @@ int check_device(int dev) {
   return 0;
 }
 
+// Drop the host-batch path's streams and buffers without freeing them: a stream
+// that cannot be synchronized may still have work on it that uses them.
+void host_path_leak(ThreadCtx &c) {
+  jnote("leak host path");
+  for (int k = 0; k < ThreadCtx::kRing; ++k) {
+    c.hstream[k] = nullptr;
+    c.dstage[k] = nullptr;
+    c.dout[k] = nullptr;
+    c.dst8[k] = c.ddesc[k] = c.hdesc[k] = nullptr;
+    c.dflag[k] = nullptr;
+  }
+  c.dbad = nullptr;
+  c.dstage_cap = c.dout_cap = 0;
+  c.zhost = c.zhost_dev = nullptr;
+  c.zhost_cap = 0;
+  c.tx_src = c.tx_dst = c.tx_desc = c.tx_hdesc = nullptr;
+  c.tx_src_cap = c.tx_dst_cap = c.tx_desc_cap = c.tx_hdesc_cap = 0;
+}
+// Wait for everything enqueued on n of the library's streams; false when that
+// failed for one of them.
+bool streams_idle(const hipStream_t *s, int n) {
+  bool idle = true;
+  for (int k = 0; k < n; ++k)
+    if (s[k] && cleared(hipStreamSynchronize(s[k])) != hipSuccess) idle = false;
+  return idle;
+}
+// rc, the result of a host-memory call, which is synchronous: on an error, what
+// the call had already enqueued is waited for, so that nothing reads the
+// caller's packets or writes its outputs after the return.
+int host_drained(int rc) {
+  if (rc && !streams_idle(t_ctx.hstream, ThreadCtx::kRing)) host_path_leak(t_ctx);
+  return rc;
+}
+
 // Free everything a context holds (on its own device; `back` is made current
 // again afterwards).  Errors are ignored: this is cleanup.
 void ctx_release(ThreadCtx &c, int back) {
@@ -2121,6 +2157,7 @@ void ctx_release(ThreadCtx &c, int back) {
   stream(c.sstream);
   hfree(c.stage);
   hfree(c.sout);
+  if (!streams_idle(c.hstream, ThreadCtx::kRing)) host_path_leak(c);
   for (int k = 0; k < ThreadCtx::kRing; ++k) {
     stream(c.hstream[k]);
     dfree(c.dstage[k]);
@@ -2135,6 +2172,8 @@ void ctx_release(ThreadCtx &c, int back) {
   dfree(c.tx_src);
   dfree(c.tx_dst);
   dfree(c.tx_desc);
+  free(c.tx_hdesc);
+  c.tx_hdesc = nullptr;
   dfree(c.rdeal);
   for (int q = 0; q < ThreadCtx::kMaxRep; ++q) {
     stream(c.rstream[q]);
@@ -4018,13 +4057,15 @@ bool aql_one_release(AqlOne &o) {
 // argument blocks, slot, streams and buffers (a pthread key destructor --
 // these run when a thread ends, not for the main thread at process exit, when
 // the runtime is being torn down anyway).  If the thread is stuck, its
-// staging buffer and result block are leaked with the rest (ctx_release then
-// skips them).
+// staging buffer, result block and burst buffer are leaked with the rest
+// (ctx_release then skips them).
 bool retire_dropins() {
   if (!aql_one_release(t_aql1)) return false;
   t_ctx.stage = t_ctx.stage_dev = nullptr;
   t_ctx.stage_cap = 0;
   t_ctx.sout = t_ctx.sout_dev = nullptr;
+  t_ctx.zhost = t_ctx.zhost_dev = nullptr;  // a burst's descriptors and outputs
+  t_ctx.zhost_cap = 0;
   return true;
 }
 
@@ -4425,10 +4466,9 @@ int mi_cksum_rx_offload(const mi_pkt_batch *b, uint32_t *csum_flags, uint32_t *c
   return launch_verify(d, batch_max_len(b), nullptr, nullptr, nullptr, bad_count, (hipStream_t)stream);
 }
 
-int mi_cksum_ipv4_verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip,
-                                uint16_t *const *l4, uint8_t *const *status, uint32_t steps,
-                                uint32_t nstreams, uint32_t timing, float *kernel_us,
-                                float *span_us) {
+static int verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip, uint16_t *const *l4,
+                         uint8_t *const *status, uint32_t steps, uint32_t nstreams, uint32_t timing,
+                         float *kernel_us, float *span_us) {
   int rc = ensure_ctx();
   if (rc) return rc;
   if (!b || !nb) return set_err(-EINVAL, "no batches");
@@ -4569,6 +4609,13 @@ int mi_cksum_ipv4_verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *co
   }
   if (span_us) *span_us = span * 1000.f;
   return 0;
+}
+int mi_cksum_ipv4_verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip, uint16_t *const *l4,
+                                uint8_t *const *status, uint32_t steps, uint32_t nstreams, uint32_t timing,
+                                float *kernel_us, float *span_us) {
+  const int rc = verify_repeat(b, nb, ip, l4, status, steps, nstreams, timing, kernel_us, span_us);
+  if (rc) (void)streams_idle(t_ctx.rstream, ThreadCtx::kMaxRep);  // (synchronous: no pass outlives an error)
+  return rc;
 }
 
 }  // extern "C"
@@ -4723,8 +4770,7 @@ int repeat_open(mi_repeat *r, uint32_t nb, uint32_t nstreams) {
 
 extern "C" {
 
-int mi_cksum_repeat_run(mi_repeat *r, uint32_t steps, uint32_t flags, float *span_us) {
-  if (!r) return set_err(-EINVAL, "handle is NULL");
+static int repeat_run(mi_repeat *r, uint32_t steps, uint32_t flags, float *span_us) {
   const bool tr = repeat_trace_on();
   if (tr) r->trace[0] = now_s();
   if (r->aql) {
@@ -4824,6 +4870,15 @@ int mi_cksum_repeat_run(mi_repeat *r, uint32_t steps, uint32_t flags, float *spa
   if (tr) r->trace[5] = now_s();
   if (timed && span_us) return mi_cksum_repeat_span(r, span_us);
   return 0;
+}
+int mi_cksum_repeat_run(mi_repeat *r, uint32_t steps, uint32_t flags, float *span_us) {
+  if (!r) return set_err(-EINVAL, "handle is NULL");
+  const int rc = repeat_run(r, steps, flags, span_us);
+  // a run that failed leaves no pass behind, an asynchronous one neither: its
+  // caller has nothing to wait for (the AQL engine's wait has a deadline, and
+  // destroying the handle leaks what a pass that missed it may still use)
+  if (rc && !r->aql) (void)streams_idle(r->s, ThreadCtx::kMaxRep);
+  return rc;
 }
 
 // Diagnostics (not in the public header): host timestamps of the last run
@@ -5222,7 +5277,7 @@ static int verify_host_zero_copy(const mi_pkt_batch *b, const uint8_t *dbase, co
   // (each a queue round trip, ~10 us apiece for a 512-packet burst).
   const size_t need = 25 * n + 128;
   if (c.zhost_cap < need) {
-    if (c.zhost) HIP_TRY(jhostfree(c.zhost));
+    if (c.zhost && !t_aql1.stuck) HIP_TRY(jhostfree(c.zhost));  // (a stuck burst may still use it)
     c.zhost = c.zhost_dev = nullptr;
     c.zhost_cap = 0;
     size_t cap = 1u << 16;
@@ -5550,18 +5605,18 @@ static int host_batch(const mi_pkt_batch *b, const HostOut &o, uint32_t *bad_cou
 
 int mi_cksum_ipv4_verify_host(const mi_pkt_batch *b, uint16_t *ip_sum, uint16_t *l4_sum,
                               uint8_t *status, uint32_t *bad_count) {
-  return host_batch(b, HostOut{ip_sum, l4_sum, status, nullptr, nullptr}, bad_count);
+  return host_drained(host_batch(b, HostOut{ip_sum, l4_sum, status, nullptr, nullptr}, bad_count));
 }
 
 int mi_cksum_rx_offload_host(const mi_pkt_batch *b, uint32_t *csum_flags, uint32_t *csum_data,
                              uint32_t *bad_count) {
   if (!csum_flags) return set_err(-EINVAL, "csum_flags is NULL");
-  return host_batch(b, HostOut{nullptr, nullptr, nullptr, csum_flags, csum_data}, bad_count);
+  return host_drained(host_batch(b, HostOut{nullptr, nullptr, nullptr, csum_flags, csum_data}, bad_count));
 }
 
 // TX copy + sums for frames in host memory (the driver's if_dpdk_transmit,
 // uinet_if_dpdk.c:583-597: socket-buffer chains -> hugepage rte_mbufs).
-int mi_cksum_tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags) {
+static int tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags) {
   HostPath host_path;  // (latency work at the TX hook: batch_activity ignores it)
   int rc = ensure_ctx();
   if (rc) return rc;
@@ -5607,7 +5662,7 @@ int mi_cksum_tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags)
   if (zc) {
     // zero-copy: descriptors and status through the mapped per-thread block
     if (c.zhost_cap < need) {
-      if (c.zhost) HIP_TRY(jhostfree(c.zhost));
+      if (c.zhost && !t_aql1.stuck) HIP_TRY(jhostfree(c.zhost));
       c.zhost = c.zhost_dev = nullptr;
       c.zhost_cap = 0;
       size_t cap = 1u << 16;
@@ -5642,11 +5697,17 @@ int mi_cksum_tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags)
   if ((rc = grow(c.tx_src, c.tx_src_cap, sbytes + 16)) || (rc = grow(c.tx_dst, c.tx_dst_cap, dbytes + 16)) ||
       (rc = grow(c.tx_desc, c.tx_desc_cap, need)))
     return rc;
-  std::vector<uint8_t> hd(need);
-  fill(hd.data());
+  if (c.tx_hdesc_cap < need) {
+    free(c.tx_hdesc);
+    c.tx_hdesc = (uint8_t *)malloc(need);
+    c.tx_hdesc_cap = c.tx_hdesc ? need : 0;
+    if (!c.tx_hdesc) return set_err(-ENOMEM, "staged TX descriptors");
+  }
+  memset(c.tx_hdesc, 0, need);
+  fill(c.tx_hdesc);
   HIP_TRY(hipMemcpyAsync(c.tx_src, b->src, b->src_bytes, hipMemcpyHostToDevice, st));
   HIP_TRY(hipMemcpyAsync(c.tx_dst, b->dst, b->dst_bytes, hipMemcpyHostToDevice, st));
-  HIP_TRY(hipMemcpyAsync(c.tx_desc, hd.data(), need, hipMemcpyHostToDevice, st));
+  HIP_TRY(hipMemcpyAsync(c.tx_desc, c.tx_hdesc, need, hipMemcpyHostToDevice, st));
   mi_tx_batch v;
   view(c.tx_desc, c.tx_src, c.tx_dst, &v);
   TxDesc t;
@@ -5656,6 +5717,9 @@ int mi_cksum_tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags)
   HIP_TRY(hipMemcpyAsync(status, c.tx_desc + o_st, n, hipMemcpyDeviceToHost, st));
   HIP_TRY(hipStreamSynchronize(st));
   return 0;
+}
+int mi_cksum_tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags) {
+  return host_drained(tx_copy_host(b, status, flags));
 }
 
 // ---------------------------------------------------------- (b1) scalar bridge

@@ -6,7 +6,8 @@
 //     stub_fail) and returned and cleared by hipGetLastError, as HIP has it;
 //   * per stream, the operations enqueued since its last synchronization;
 //   * the live allocations, and frees of memory that is not one of them.
-// stub_fail(name, nth, err): the nth call of that function from now on fails.
+// stub_fail(name, nth, err): the nth call of that function from now on fails
+// (stub_fail_from: every call from the nth on).
 #include <hip/hip_runtime_api.h>
 
 #include <stdint.h>
@@ -25,6 +26,7 @@ std::mutex g_mu;
 struct Fail {
   int nth = 0;
   hipError_t err = hipSuccess;
+  bool all = false;  // every call from the nth on
 };
 std::map<std::string, Fail> g_fail;
 std::map<std::string, int> g_calls;
@@ -45,7 +47,7 @@ hipError_t enter(const char *name) {
   auto it = g_fail.find(name);
   if (it == g_fail.end() || --it->second.nth > 0) return hipSuccess;
   const hipError_t e = it->second.err;
-  g_fail.erase(it);
+  if (!it->second.all) g_fail.erase(it);
   return e;
 }
 #define ENTER(name)                          \
@@ -81,6 +83,10 @@ void stub_fail(const char *name, int nth, int err) {
   std::lock_guard<std::mutex> lk(g_mu);
   g_fail[name] = Fail{nth, (hipError_t)err};
 }
+void stub_fail_from(const char *name, int nth, int err) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  g_fail[name] = Fail{nth, (hipError_t)err, true};
+}
 void stub_set_last(int err) { t_last = (hipError_t)err; }
 int stub_last(void) { return (int)t_last; }
 // Every function called since the last stub_reset, as "name count" lines.
@@ -102,10 +108,12 @@ int stub_calls(const char *name) {
   std::lock_guard<std::mutex> lk(g_mu);
   return g_calls[name];
 }
-int stub_pending(void) {
+// In flight on the streams the library made (own) / on the default stream.
+int stub_pending(int own) {
   std::lock_guard<std::mutex> lk(g_mu);
   int n = 0;
-  for (auto &p : g_pending) n += p.second;
+  for (auto &p : g_pending)
+    if ((p.first != nullptr) == (own != 0)) n += p.second;
   return n;
 }
 int stub_live(void) {

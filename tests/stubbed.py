@@ -19,7 +19,7 @@ import numpy as np
 
 ROOT, STUB = sys.argv[1], sys.argv[2]
 stub = C.CDLL(STUB, mode=C.RTLD_GLOBAL)  # ahead of the library: its symbols win
-stub.stub_fail.argtypes = [C.c_char_p, C.c_int, C.c_int]
+stub.stub_fail.argtypes = stub.stub_fail_from.argtypes = [C.c_char_p, C.c_int, C.c_int]
 spec = importlib.util.spec_from_file_location("_lib", os.path.join(ROOT, "libunsod_amd", "_lib.py"))
 _lib = importlib.util.module_from_spec(spec)
 spec.loader.exec_module(_lib)

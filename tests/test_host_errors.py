@@ -217,3 +217,37 @@ def check(where, call, rc):
 
 assert sweep(check) > 200
 ''', MI_CKSUM_HOST_CHUNK="20000")
+
+
+def test_no_error_return_leaves_work_in_flight(so):
+    """Whatever runtime call fails, a call that runs on the library's own streams
+    returns with nothing on them: a host-memory batch (several chunks), a
+    back-to-back submission, a handle's run."""
+    stubbed.run(so, SWEEP + r'''
+def check(where, call, rc):
+    assert stub.stub_pending(1) == 0, (where, rc)
+
+
+assert sweep(check) > 200
+''', MI_CKSUM_HOST_CHUNK="20000")
+
+
+def test_what_cannot_be_waited_for_is_not_freed(so):
+    """A host batch fails and its streams cannot be synchronized: the buffers
+    that its kernels may still use are neither freed nor used again, and the
+    next call works with others."""
+    stubbed.run(so, SWEEP + r'''
+for name in ("verify_host", "verify_host, lengths", "rx_offload_host", "tx_copy_host", "verify_host, registered"):
+    def one():
+        call = entries[name]
+        assert call() == 0, err()
+        live = stub.stub_live()
+        fail("hipLaunchKernel")
+        stub.stub_fail_from(b"hipStreamSynchronize", 1 + (name not in ("tx_copy_host", "verify_host, registered")), INVALID)
+        assert call() == EIO, name
+        stub.stub_reset()
+        assert stub.stub_live() == live, name
+        assert call() == 0, (name, err())
+        assert stub.stub_live() > live and calls("hipFree") + calls("hipHostFree") == 0, name
+    in_thread(one)
+''', MI_CKSUM_HOST_CHUNK="20000")
