@@ -4537,29 +4537,41 @@ static int verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip
       }
       HIP_TRY(hipStreamSynchronize(c.rstream[0]));
       HIP_TRY(hipStreamBeginCapture(c.rstream[0], hipStreamCaptureModeThreadLocal));
-      HIP_TRY(hipEventRecord(c.rfork, c.rstream[0]));
-      for (uint32_t q = 1; q < nstreams; ++q) HIP_TRY(hipStreamWaitEvent(c.rstream[q], c.rfork, 0));
-      for (uint32_t k = 0; k < steps && !rc; ++k) {
-        const uint32_t j = k % nb;
-        rc = launch_verify(d[j], ml[j], ip ? ip[j] : nullptr, l4 ? l4[j] : nullptr,
-                           status ? status[j] : nullptr, nullptr, c.rstream[k % nstreams], deal_set(k % nstreams));
-      }
-      for (uint32_t q = 1; q < nstreams; ++q) {
-        HIP_TRY(hipEventRecord(c.rjoin[q], c.rstream[q]));
-        HIP_TRY(hipStreamWaitEvent(c.rstream[0], c.rjoin[q], 0));
-      }
+      auto record = [&]() -> int {
+        HIP_TRY(hipEventRecord(c.rfork, c.rstream[0]));
+        for (uint32_t q = 1; q < nstreams; ++q) HIP_TRY(hipStreamWaitEvent(c.rstream[q], c.rfork, 0));
+        for (uint32_t k = 0; k < steps; ++k) {
+          const uint32_t j = k % nb;
+          const int lrc = launch_verify(d[j], ml[j], ip ? ip[j] : nullptr, l4 ? l4[j] : nullptr,
+                                        status ? status[j] : nullptr, nullptr, c.rstream[k % nstreams],
+                                        deal_set(k % nstreams));
+          if (lrc) return lrc;
+        }
+        for (uint32_t q = 1; q < nstreams; ++q) {
+          HIP_TRY(hipEventRecord(c.rjoin[q], c.rstream[q]));
+          HIP_TRY(hipStreamWaitEvent(c.rstream[0], c.rjoin[q], 0));
+        }
+        return 0;
+      };
+      // (ended whether the recording worked or not: a stream left capturing
+      // refuses every later call)
+      rc = record();
       hipGraph_t g = nullptr;
-      HIP_TRY(hipStreamEndCapture(c.rstream[0], &g));
+      const hipError_t ce = cleared(hipStreamEndCapture(c.rstream[0], &g));
+      if (!rc && ce != hipSuccess) rc = set_err(-EIO, "hipStreamEndCapture: %s", hipGetErrorString(ce));
       if (rc) {
-        (void)cleared(hipGraphDestroy(g));
+        if (g) (void)cleared(hipGraphDestroy(g));
         return rc;
       }
       gr = &c.rgraph[c.rgraph_next];
       c.rgraph_next = (c.rgraph_next + 1) % ThreadCtx::kGraphs;
       if (gr->exec) (void)cleared(hipGraphExecDestroy(gr->exec));
       gr->exec = nullptr;
-      HIP_TRY(hipGraphInstantiate(&gr->exec, g, nullptr, nullptr, 0));
+      hipGraphExec_t exec = nullptr;
+      const hipError_t ie = cleared(hipGraphInstantiate(&exec, g, nullptr, nullptr, 0));
       (void)cleared(hipGraphDestroy(g));
+      if (ie != hipSuccess) return set_err(-EIO, "hipGraphInstantiate: %s", hipGetErrorString(ie));
+      gr->exec = exec;
       gr->key = key;
       gr->steps = steps;
       gr->nstreams = nstreams;

@@ -55,7 +55,9 @@ hipError_t enter(const char *name) {
     const hipError_t e_ = enter(name);       \
     if (e_ != hipSuccess) return ret(e_);    \
   } while (0)
+bool capturing();
 void enqueue(void *s) {
+  if (capturing()) return;
   std::lock_guard<std::mutex> lk(g_mu);
   ++g_pending[s];
 }
@@ -254,6 +256,7 @@ hipError_t hipMemcpy2DAsync(void *d, size_t dp, const void *s, size_t sp, size_t
   return hipSuccess;
 }
 
+int stub_capturing(void);
 hipError_t hipStreamCreateWithFlags(hipStream_t *s, unsigned) {
   ENTER("hipStreamCreateWithFlags");
   *s = (hipStream_t)malloc(16);
@@ -266,6 +269,7 @@ hipError_t hipStreamDestroy(hipStream_t s) {
 }
 hipError_t hipStreamSynchronize(hipStream_t s) {
   ENTER("hipStreamSynchronize");
+  if (stub_capturing()) return ret(hipErrorStreamCaptureUnsupported);
   std::lock_guard<std::mutex> lk(g_mu);
   g_pending[s] = 0;
   return hipSuccess;
@@ -304,6 +308,56 @@ hipError_t hipEventElapsedTime(float *ms, hipEvent_t, hipEvent_t) {
   return hipSuccess;
 }
 
+// Stream capture: one at a time; while it lasts, launches are recorded (not in
+// flight) and its stream cannot be synchronized.
+static hipStream_t g_capturing = nullptr;
+static int g_graphs = 0;  // graphs and executables not destroyed
+int stub_capturing(void) { return g_capturing != nullptr; }
+int stub_graphs(void) { return g_graphs; }
+hipError_t hipStreamBeginCapture(hipStream_t s, hipStreamCaptureMode) {
+  ENTER("hipStreamBeginCapture");
+  if (g_capturing) return ret(hipErrorIllegalState);
+  g_capturing = s;
+  return hipSuccess;
+}
+hipError_t hipStreamEndCapture(hipStream_t s, hipGraph_t *g) {
+  const hipError_t e = enter("hipStreamEndCapture");  // (a failed one ends the capture too)
+  *g = nullptr;
+  if (g_capturing != s) return ret(hipErrorIllegalState);
+  g_capturing = nullptr;
+  if (e != hipSuccess) return ret(e);
+  *g = (hipGraph_t)malloc(16);
+  ++g_graphs;
+  return hipSuccess;
+}
+hipError_t hipGraphDestroy(hipGraph_t g) {
+  ENTER("hipGraphDestroy");
+  free(g);
+  --g_graphs;
+  return hipSuccess;
+}
+hipError_t hipGraphInstantiate(hipGraphExec_t *x, hipGraph_t, hipGraphNode_t *, char *, size_t) {
+  ENTER("hipGraphInstantiate");
+  *x = (hipGraphExec_t)malloc(16);
+  ++g_graphs;
+  return hipSuccess;
+}
+hipError_t hipGraphExecDestroy(hipGraphExec_t x) {
+  ENTER("hipGraphExecDestroy");
+  free(x);
+  --g_graphs;
+  return hipSuccess;
+}
+hipError_t hipGraphUpload(hipGraphExec_t, hipStream_t) {
+  ENTER("hipGraphUpload");
+  return hipSuccess;
+}
+hipError_t hipGraphLaunch(hipGraphExec_t, hipStream_t s) {
+  ENTER("hipGraphLaunch");
+  enqueue(s);
+  return hipSuccess;
+}
+
 // kernel<<<>>>: the configuration pushed here is popped by the kernel's host
 // stub, which then calls hipLaunchKernel.
 struct LaunchConfig {
@@ -334,3 +388,7 @@ hipError_t hipExtLaunchKernel(const void *, dim3, dim3, void **, size_t, hipStre
   return hipSuccess;
 }
 }
+
+namespace {
+bool capturing() { return g_capturing != nullptr; }
+}  // namespace

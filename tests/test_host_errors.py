@@ -153,6 +153,7 @@ entries = {
     "verify_host, registered": lambda: registered(chunked),
     "verify_repeat": lambda: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, 2, 1, None, us),
     "verify_repeat, per pass": lambda: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, 2, 2, us, None),
+    "verify_repeat, graph": lambda: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, 2, 0x101, None, us),
     "repeat handle": whole,
     "tx repeat handle": lambda: whole(True),
     "drop-in staging": lambda: 0 if lib.mi__scalar_staging(100) else -1,
@@ -250,4 +251,29 @@ for name in ("verify_host", "verify_host, lengths", "rx_offload_host", "tx_copy_
         assert call() == 0, (name, err())
         assert stub.stub_live() > live and calls("hipFree") + calls("hipHostFree") == 0, name
     in_thread(one)
+''', MI_CKSUM_HOST_CHUNK="20000")
+
+
+def test_an_error_inside_a_capture_ends_it(so):
+    """A back-to-back submission as a graph whose recording fails leaves no
+    stream capturing and no graph behind, and the next submission works."""
+    stubbed.run(so, SWEEP + r'''
+import time
+
+entries = {"verify_repeat, graph": entries["verify_repeat, graph"]}
+leaked = [0]  # graphs whose destruction was made to fail
+
+
+def check(where, call, rc):
+    assert not stub.stub_capturing(), (where, rc, err())
+    t0 = time.monotonic()  # (the previous thread's context goes just after the thread)
+    while stub.stub_graphs() > leaked[0] + 1 and time.monotonic() < t0 + 1.0:
+        time.sleep(0.001)
+    leaked[0] += where[1] == "hipGraphDestroy"
+    assert stub.stub_graphs() <= leaked[0] + 1, (where, stub.stub_graphs())
+    stub.stub_reset()
+    assert call() == 0 and stub.stub_pending(1) == 0, (where, err())
+
+
+assert sweep(check) > 20
 ''', MI_CKSUM_HOST_CHUNK="20000")
