@@ -1961,12 +1961,14 @@ template <typename T>
 hipError_t jmalloc(T **p, size_t n) {
   const hipError_t e = cleared(hipMalloc((void **)p, n));
   if (e == hipSuccess) jnote("alloc device", *p, n);
+  else *p = nullptr;
   return e;
 }
 template <typename T>
 hipError_t jhostmalloc(T **p, size_t n, unsigned flags) {
   const hipError_t e = cleared(hipHostMalloc((void **)p, n, flags));
   if (e == hipSuccess) jnote("alloc host", *p, n);
+  else *p = nullptr;
   return e;
 }
 hipError_t jfree(void *p) {
@@ -1976,6 +1978,25 @@ hipError_t jfree(void *p) {
 hipError_t jhostfree(void *p) {
   if (p) jnote("free host", p, alloc_bytes(p));
   return cleared(hipHostFree(p));
+}
+// p, a buffer or null, replaced by one of n bytes.  Null when either step
+// fails: a capacity kept beside several buffers is 0 while they are regrown, so
+// that a later, smaller call does not take one that is gone.
+template <typename T>
+int regrow(T *&p, size_t n) {
+  T *const old = p;
+  p = nullptr;
+  if (old) HIP_TRY(jfree(old));
+  HIP_TRY(jmalloc(&p, n));
+  return 0;
+}
+template <typename T>
+int regrow_host(T *&p, size_t n) {
+  T *const old = p;
+  p = nullptr;
+  if (old) HIP_TRY(jhostfree(old));
+  HIP_TRY(jhostmalloc(&p, n, hipHostMallocDefault));
+  return 0;
 }
 hsa_status_t fault_event(const hsa_amd_event_t *ev, void *) {
   if (!ev || ev->event_type != HSA_AMD_GPU_MEMORY_FAULT_EVENT) return HSA_STATUS_SUCCESS;
@@ -2118,6 +2139,13 @@ void host_path_leak(ThreadCtx &c) {
   c.zhost_cap = 0;
   c.tx_src = c.tx_dst = c.tx_desc = c.tx_hdesc = nullptr;
   c.tx_src_cap = c.tx_dst_cap = c.tx_desc_cap = c.tx_hdesc_cap = 0;
+}
+// The host-batch path's streams, each created once (a call that failed half way
+// through left the rest to the next one).
+int host_streams(ThreadCtx &c) {
+  for (hipStream_t &s : c.hstream)
+    if (!s) HIP_TRY(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+  return 0;
 }
 // Wait for everything enqueued on n of the library's streams; false when that
 // failed for one of them.
@@ -4500,8 +4528,14 @@ static int verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip
   }
   if (!c.rgate) HIP_TRY(hipEventCreateWithFlags(&c.rgate, hipEventDisableTiming));
   if (!c.rdeal && deal_on()) {
-    HIP_TRY(jmalloc(&c.rdeal, (size_t)kDealSetBytes * ThreadCtx::kMaxRep));
-    HIP_TRY(hipMemset(c.rdeal, 0, (size_t)kDealSetBytes * ThreadCtx::kMaxRep));
+    uint32_t *sets = nullptr;
+    HIP_TRY(jmalloc(&sets, (size_t)kDealSetBytes * ThreadCtx::kMaxRep));
+    const hipError_t e = cleared(hipMemset(sets, 0, (size_t)kDealSetBytes * ThreadCtx::kMaxRep));
+    if (e != hipSuccess) {
+      (void)jfree(sets);
+      return set_err(-EIO, "deal counters: %s", hipGetErrorString(e));
+    }
+    c.rdeal = sets;
   }
   auto deal_set = [&](uint32_t q) { return c.rdeal ? c.rdeal + q * (kDealSetBytes / 4u) : nullptr; };
   const bool graph = timing & MI_REPEAT_GRAPH;
@@ -4531,10 +4565,9 @@ static int verify_repeat(const mi_pkt_batch *b, uint32_t nb, uint16_t *const *ip
     for (auto &e : c.rgraph)
       if (e.exec && e.key == key && e.steps == steps && e.nstreams == nstreams) gr = &e;
     if (!gr) {
-      if (!c.rfork) {
-        HIP_TRY(hipEventCreateWithFlags(&c.rfork, hipEventDisableTiming));
-        for (int q = 0; q < ThreadCtx::kMaxRep; ++q) HIP_TRY(hipEventCreateWithFlags(&c.rjoin[q], hipEventDisableTiming));
-      }
+      if (!c.rfork) HIP_TRY(hipEventCreateWithFlags(&c.rfork, hipEventDisableTiming));
+      for (hipEvent_t &e : c.rjoin)
+        if (!e) HIP_TRY(hipEventCreateWithFlags(&e, hipEventDisableTiming));
       HIP_TRY(hipStreamSynchronize(c.rstream[0]));
       HIP_TRY(hipStreamBeginCapture(c.rstream[0], hipStreamCaptureModeThreadLocal));
       auto record = [&]() -> int {
@@ -5189,9 +5222,15 @@ extern "C" int mi__reg_table_count(void) {
 static int ensure_sout(ThreadCtx &c) {
   if (c.sout) return 0;
   // words 0..5: the result and the trace stamps (kOutWords)
-  HIP_TRY(jhostmalloc((void **)&c.sout, 4096, hipHostMallocMapped | hipHostMallocCoherent));
-  HIP_TRY(hipHostGetDevicePointer((void **)&c.sout_dev, c.sout, 0));
-  memset(c.sout, 0, 4096);
+  uint32_t *out = nullptr;
+  HIP_TRY(jhostmalloc(&out, 4096, hipHostMallocMapped | hipHostMallocCoherent));
+  const hipError_t e = cleared(hipHostGetDevicePointer((void **)&c.sout_dev, out, 0));
+  if (e != hipSuccess) {  // (c.sout stays null: the next call tries again)
+    (void)jhostfree(out);
+    return set_err(-EIO, "result block: %s", hipGetErrorString(e));
+  }
+  memset(out, 0, 4096);
+  c.sout = out;
   dbg_mem("sout", c.sout_dev, 4096);
   return 0;
 }
@@ -5422,12 +5461,11 @@ static int verify_host_zero_copy(const mi_pkt_batch *b, const uint8_t *dbase, co
   } else {
     // (the HIP fallback: its streams only now -- a stream may create a queue,
     // which shifts the library's queue placement, place_*)
-    if (!c.hstream[0])
-      for (int k = 0; k < ThreadCtx::kRing; ++k)
-        HIP_TRY(hipStreamCreateWithFlags(&c.hstream[k], hipStreamNonBlocking));
+    int rc = host_streams(c);
+    if (rc) return rc;
     hipStream_t st = c.hstream[0];
-    int rc = wide ? launch_verify_shape(d, Shape{64, 4}, zip, zl4, zst, zbad, st)
-                  : launch_verify(d, max_len, zip, zl4, zst, zbad, st);
+    rc = wide ? launch_verify_shape(d, Shape{64, 4}, zip, zl4, zst, zbad, st)
+              : launch_verify(d, max_len, zip, zl4, zst, zbad, st);
     if (rc) return rc;
     HIP_TRY(hipStreamSynchronize(st));
   }
@@ -5512,30 +5550,21 @@ static int host_batch(const mi_pkt_batch *b, const HostOut &o, uint32_t *bad_cou
   need_stage = (need_stage + 64) & ~15ull;
   if (need_stage > kMaxBytes) return set_err(-E2BIG, "packet too large for staging");
 
-  if (!c.hstream[0])
-    for (int k = 0; k < ThreadCtx::kRing; ++k)
-      HIP_TRY(hipStreamCreateWithFlags(&c.hstream[k], hipStreamNonBlocking));
+  if ((rc = host_streams(c))) return rc;
   if (!c.dbad) HIP_TRY(jmalloc(&c.dbad, 4 * ThreadCtx::kRing));
   if (c.dstage_cap < need_stage) {
-    for (int k = 0; k < ThreadCtx::kRing; ++k) {
-      if (c.dstage[k]) HIP_TRY(jfree(c.dstage[k]));
-      HIP_TRY(jmalloc(&c.dstage[k], need_stage));
-    }
+    c.dstage_cap = 0;
+    for (int k = 0; k < ThreadCtx::kRing; ++k)
+      if ((rc = regrow(c.dstage[k], need_stage))) return rc;
     c.dstage_cap = need_stage;
   }
   if (c.dout_cap < max_pk) {
-    for (int k = 0; k < ThreadCtx::kRing; ++k) {
-      if (c.dout[k]) HIP_TRY(jfree(c.dout[k]));
-      if (c.dst8[k]) HIP_TRY(jfree(c.dst8[k]));
-      if (c.ddesc[k]) HIP_TRY(jfree(c.ddesc[k]));
-      if (c.hdesc[k]) HIP_TRY(jhostfree(c.hdesc[k]));
-      if (c.dflag[k]) HIP_TRY(jfree(c.dflag[k]));
-      HIP_TRY(jmalloc(&c.dflag[k], 8ull * max_pk));
-      HIP_TRY(jmalloc(&c.dout[k], 4ull * max_pk));
-      HIP_TRY(jmalloc(&c.dst8[k], (size_t)max_pk + 16));
-      HIP_TRY(jmalloc(&c.ddesc[k], 12ull * max_pk));
-      HIP_TRY(jhostmalloc((void **)&c.hdesc[k], 12ull * max_pk, hipHostMallocDefault));
-    }
+    c.dout_cap = 0;
+    for (int k = 0; k < ThreadCtx::kRing; ++k)
+      if ((rc = regrow(c.dflag[k], 8ull * max_pk)) || (rc = regrow(c.dout[k], 4ull * max_pk)) ||
+          (rc = regrow(c.dst8[k], (size_t)max_pk + 16)) || (rc = regrow(c.ddesc[k], 12ull * max_pk)) ||
+          (rc = regrow_host(c.hdesc[k], 12ull * max_pk)))
+        return rc;
     c.dout_cap = max_pk;
   }
   HIP_TRY(hipMemsetAsync(c.dbad, 0, 4 * ThreadCtx::kRing, c.hstream[0]));
@@ -5662,8 +5691,7 @@ static int tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags) {
     v->csum_flags = b->csum_flags ? (const uint32_t *)(z + o_cf) : nullptr;
     v->csum_data = b->csum_data ? (const uint32_t *)(z + o_cd) : nullptr;
   };
-  if (!c.hstream[0])
-    for (int k = 0; k < ThreadCtx::kRing; ++k) HIP_TRY(hipStreamCreateWithFlags(&c.hstream[k], hipStreamNonBlocking));
+  if ((rc = host_streams(c))) return rc;
   hipStream_t st = c.hstream[0];
   const Shape sh = pick_tx_shape(b->max_len ? b->max_len : b->room);
   void *sdev = nullptr, *ddev = nullptr;
@@ -5698,12 +5726,10 @@ static int tx_copy_host(const mi_tx_batch *b, uint8_t *status, uint32_t flags) {
   if (!b->src || !b->dst) return set_err(-EINVAL, "NULL array");
   auto grow = [&](uint8_t *&p, size_t &cap, size_t want) -> int {
     if (cap >= want) return 0;
-    if (p) HIP_TRY(jfree(p));
-    p = nullptr;
     cap = 0;
-    HIP_TRY(jmalloc((void **)&p, want));
-    cap = want;
-    return 0;
+    const int grc = regrow(p, want);
+    if (!grc) cap = want;
+    return grc;
   };
   const size_t sbytes = (b->src_bytes + 15u) & ~15ull, dbytes = (b->dst_bytes + 15u) & ~15ull;
   if ((rc = grow(c.tx_src, c.tx_src_cap, sbytes + 16)) || (rc = grow(c.tx_dst, c.tx_dst_cap, dbytes + 16)) ||

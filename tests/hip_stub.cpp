@@ -5,7 +5,8 @@
 //   * the calling thread's last error, set by every call that fails (here or by
 //     stub_fail) and returned and cleared by hipGetLastError, as HIP has it;
 //   * per stream, the operations enqueued since its last synchronization;
-//   * the live allocations, and frees of memory that is not one of them.
+//   * the live allocations, frees of memory that is not one of them, and copies
+//     whose device side does not lie inside one.
 // stub_fail(name, nth, err): the nth call of that function from now on fails
 // (stub_fail_from: every call from the nth on).
 #include <hip/hip_runtime_api.h>
@@ -33,7 +34,7 @@ std::map<std::string, int> g_calls;
 std::map<void *, int> g_pending;  // stream -> operations in flight
 std::map<void *, size_t> g_live;
 std::map<void *, size_t> g_registered;
-int g_bad_frees = 0;
+int g_bad_frees = 0, g_bad_copies = 0;
 std::atomic<int> g_errors{0};
 
 hipError_t ret(hipError_t e) {
@@ -60,6 +61,17 @@ void enqueue(void *s) {
   if (capturing()) return;
   std::lock_guard<std::mutex> lk(g_mu);
   ++g_pending[s];
+}
+// Does [p, p + n) lie inside a live allocation?  Counted if not.
+bool on_device(const void *p, size_t n) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  for (auto &a : g_live)
+    if ((char *)p >= (char *)a.first && (char *)p + n <= (char *)a.first + a.second) return true;
+  ++g_bad_copies;
+  return false;
+}
+bool copy_ok(const void *d, const void *s, size_t n, hipMemcpyKind k) {
+  return n == 0 || on_device(k == hipMemcpyHostToDevice ? d : s, n);
 }
 hipError_t alloc(void **p, size_t n) {
   *p = aligned_alloc(4096, (n + 8191) & ~(size_t)4095);
@@ -128,6 +140,7 @@ int stub_registered(void) {
 }
 int stub_errors(void) { return g_errors; }
 int stub_bad_frees(void) { return g_bad_frees; }
+int stub_bad_copies(void) { return g_bad_copies; }
 
 hipError_t hipGetLastError(void) {
   const hipError_t e = t_last;
@@ -237,20 +250,23 @@ hipError_t hipMemsetAsync(void *p, int v, size_t n, hipStream_t s) {
   enqueue(s);
   return hipSuccess;
 }
-hipError_t hipMemcpy(void *d, const void *s, size_t n, hipMemcpyKind) {
+hipError_t hipMemcpy(void *d, const void *s, size_t n, hipMemcpyKind k) {
   ENTER("hipMemcpy");
+  if (!copy_ok(d, s, n, k)) return ret(hipErrorInvalidValue);
   memcpy(d, s, n);
   return hipSuccess;
 }
-hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, hipMemcpyKind, hipStream_t st) {
+hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, hipMemcpyKind k, hipStream_t st) {
   ENTER("hipMemcpyAsync");
+  if (!copy_ok(d, s, n, k)) return ret(hipErrorInvalidValue);
   memcpy(d, s, n);
   enqueue(st);
   return hipSuccess;
 }
-hipError_t hipMemcpy2DAsync(void *d, size_t dp, const void *s, size_t sp, size_t w, size_t h, hipMemcpyKind,
+hipError_t hipMemcpy2DAsync(void *d, size_t dp, const void *s, size_t sp, size_t w, size_t h, hipMemcpyKind k,
                             hipStream_t st) {
   ENTER("hipMemcpy2DAsync");
+  if (h && !copy_ok(d, s, (h - 1) * (k == hipMemcpyHostToDevice ? dp : sp) + w, k)) return ret(hipErrorInvalidValue);
   for (size_t r = 0; r < h; ++r) memcpy((char *)d + r * dp, (const char *)s + r * sp, w);
   enqueue(st);
   return hipSuccess;
@@ -275,8 +291,9 @@ hipError_t hipStreamSynchronize(hipStream_t s) {
   return hipSuccess;
 }
 hipError_t hipStreamQuery(hipStream_t s) { return hipStreamSynchronize(s); }
-hipError_t hipStreamWaitEvent(hipStream_t, hipEvent_t, unsigned) {
+hipError_t hipStreamWaitEvent(hipStream_t, hipEvent_t e, unsigned) {
   ENTER("hipStreamWaitEvent");
+  if (!e) return ret(hipErrorInvalidHandle);
   return hipSuccess;
 }
 hipError_t hipEventCreate(hipEvent_t *e) {
@@ -290,8 +307,9 @@ hipError_t hipEventDestroy(hipEvent_t e) {
   free(e);
   return hipSuccess;
 }
-hipError_t hipEventRecord(hipEvent_t, hipStream_t) {
+hipError_t hipEventRecord(hipEvent_t e, hipStream_t) {
   ENTER("hipEventRecord");
+  if (!e) return ret(hipErrorInvalidHandle);
   return hipSuccess;
 }
 hipError_t hipEventQuery(hipEvent_t) {

@@ -277,3 +277,84 @@ def check(where, call, rc):
 
 assert sweep(check) > 20
 ''', MI_CKSUM_HOST_CHUNK="20000")
+
+
+def test_a_call_after_a_failed_one_works(so):
+    """Whatever runtime call fails while a context is set up or regrown, a
+    smaller and then the same call after it work: on the library's own streams,
+    in buffers that are there and large enough, nothing freed twice."""
+    body = r'''
+big = batch(4 * n, stride=4096)
+o16, o8, o32 = np.zeros(8 * n, np.uint16), np.zeros(4 * n, np.uint8), np.zeros(8 * n, np.uint32)
+p16, p8, p32 = o16.ctypes.data, o8.ctypes.data, o32.ctypes.data
+blens = np.full(4 * n, 1500, np.uint32)
+bmixed, btb = batch(4 * n, lens=blens), tx_batch(64)
+bad = C.byref(C.c_uint32())
+sized = {  # name: (a small call, a larger one)
+    "verify_host": [lambda x=x: lib.mi_cksum_ipv4_verify_host(C.byref(x), p16, p16 + 8 * n, p8, bad) for x in (b, big)],
+    "verify_host, lengths": [lambda x=x: lib.mi_cksum_ipv4_verify_host(C.byref(x), p16, None, p8, bad)
+                             for x in (mixed, bmixed)],
+    "rx_offload_host": [lambda x=x: lib.mi_cksum_rx_offload_host(C.byref(x), p32, p32 + 16 * n, bad) for x in (b, bmixed)],
+    "tx_copy_host": [lambda x=x: lib.mi_cksum_tx_copy_host(C.byref(x), p8, 0) for x in (tb, btb)],
+    "verify_repeat": [lambda k=k: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, k, 1, None, us)
+                      for k in (1, 4)],
+    "verify_repeat, graph": [lambda k=k: lib.mi_cksum_ipv4_verify_repeat(B, 1, None, None, st1, 3, k, 0x101, None, us)
+                             for k in (1, 4)],
+}
+memsets = os.environ.get("MI_CKSUM_DEAL") == "1"
+for name, (small, large) in sized.items():
+    for first in (None, small):  # a fresh context; one that has to grow
+        def grown():
+            if first:
+                assert first() == 0, err()
+            stub.stub_reset()
+            assert large() == 0, err()
+            return dict((k, int(v)) for k, v in (ln.split() for ln in stub.stub_counts().decode().splitlines()))
+        for fn, k in in_thread(grown).items():
+            for nth in range(1, k + 1):
+                def one():
+                    if first:
+                        assert first() == 0, err()
+                    stub.stub_reset()
+                    fail(fn, nth, NOMEM)
+                    before = stub.stub_pending(0)
+                    rc = large()
+                    stub.stub_reset()
+                    for again in (small, large):
+                        assert again() == 0, (name, bool(first), fn, nth, rc, err())
+                    assert stub.stub_pending(0) == before, (name, fn, nth, "the default stream")
+                    if memsets and name == "verify_repeat" and fn == "hipMemset" and rc:
+                        assert calls("hipMemset") == 1, "the counters were never cleared"
+                in_thread(one)
+assert stub.stub_bad_copies() == 0 and stub.stub_bad_frees() == 0
+'''
+    stubbed.run(so, SWEEP + body, MI_CKSUM_HOST_CHUNK="20000")
+    stubbed.run(so, SWEEP + body, MI_CKSUM_HOST_CHUNK="20000", MI_CKSUM_DEAL="1")
+
+
+def test_a_result_block_without_a_device_address_is_not_kept(so):
+    """The drop-ins' result block: a failed address query is asked again by the
+    next call, whose kernel would otherwise store through a null address."""
+    stubbed.run(so, r'''
+hdr = (C.c_uint8 * 20)(*bytes.fromhex("450000730000400040110000c0a80001c0a800c7"))
+lib.mi_cksum_set_dropin_mode(1)
+assert lib.in_cksum_hdr(hdr) in (0x61b8, 0xb861)  # (no kernel runs here: answered by the host fold)
+import threading
+seen = []
+
+
+def go():
+    lib.in_cksum_hdr.restype = C.c_uint
+    for k in range(2):
+        stub.stub_reset()
+        fail("hipHostGetDevicePointer", 2 if k == 0 else 99)
+        lib.in_cksum_hdr(hdr)
+        seen.append((calls("hipHostGetDevicePointer"), calls("hipLaunchKernel")))
+
+
+t = threading.Thread(target=go)
+t.start()
+t.join()
+# first call: staging, then the block, refused: no kernel; second: the block again, a kernel
+assert seen == [(2, 0), (1, 1)], seen
+''')
