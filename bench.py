@@ -22,6 +22,7 @@ path.  Prints ONE JSON line.
 from __future__ import annotations
 
 import argparse
+import errno
 import json
 import os
 import sys
@@ -829,8 +830,10 @@ def host_path(mi, host: np.ndarray, n: int, L_sum: int, lay: dict, iters: int = 
     pinned = True
     try:
         mi.host_register(host)
-    except Exception:
-        pinned = False
+    except mi.MiCksumError as e:
+        if e.rc != -errno.ENOTSUP:
+            raise
+        pinned = False  # not page-locked here: both rates are the staged path's
 
     def rate(staged: bool):
         mi.ipv4_verify_host(host, n, staged=staged, **lay)

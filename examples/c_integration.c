@@ -9,13 +9,15 @@
  *      application threads and the callout thread concurrently), folded on
  *      the CPU (the default) and through the GPU drop-in service.
  *   2. (b2) a host-memory RX burst as the DPDK driver holds it (rte_mbuf slots
- *      of 2176 B, IP header at +142): TX-finalized, registered, verified in
- *      place over PCIe, then one corrupted datagram detected.
+ *      of 2176 B, IP header at +142): TX-finalized, registered and verified in
+ *      place over PCIe (staged where registration is not supported), then one
+ *      corrupted datagram detected.
  *
  * Built by libunsod_amd/csrc/Makefile (into libunsod_amd/lib/) with plain gcc:
  *   gcc -O2 -pthread -Iinclude examples/c_integration.c -Llibunsod_amd/lib -lmicksum
  * Prints "c_integration ok" and exits 0 when every check holds.
  */
+#include <errno.h>
 #include <pthread.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -177,14 +179,19 @@ int main(void)
 	uint16_t *ip_sum = calloc(n, 2), *l4_sum = calloc(n, 2);
 	uint8_t *status = calloc(n, 1);
 	uint32_t bad = 0;
-	/* page-lock + map the pool once: the verify kernel then reads it in place */
-	CHECK(mi_cksum_host_register(pool, alloc) == 0, "register: %s", mi_cksum_strerror());
+	/* page-lock + map the pool once: the verify kernel then reads it in place.
+	 * Where the system does not lock memory that already exists (-ENOTSUP) the
+	 * same calls copy the burst through device staging. */
+	const int reg = mi_cksum_host_register(pool, alloc);
+	CHECK(reg == 0 || reg == -ENOTSUP, "register: %s", mi_cksum_strerror());
+	printf("burst: %s\n", reg == 0 ? "read in place" : "staged");
 	CHECK(mi_cksum_ipv4_verify_host(&b, ip_sum, l4_sum, status, &bad) == 0, "verify_host: %s", mi_cksum_strerror());
 	CHECK(bad == 0, "valid burst: %u bad", bad);
 	pool[first + 777u * stride + 900] ^= 0x10;
 	CHECK(mi_cksum_ipv4_verify_host(&b, ip_sum, l4_sum, status, &bad) == 0, "verify_host: %s", mi_cksum_strerror());
 	CHECK(bad == 1 && status[777] == MI_ST_L4_BAD, "corrupted datagram: bad %u status %u", bad, status[777]);
-	mi_cksum_host_unregister(pool);
+	if (reg == 0)
+		CHECK(mi_cksum_host_unregister(pool) == 0, "unregister: %s", mi_cksum_strerror());
 	free(pool);
 	free(ip_sum);
 	free(l4_sum);

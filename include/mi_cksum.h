@@ -537,7 +537,12 @@ int mi_cksum_rx_offload_host(const mi_pkt_batch *b, uint32_t *csum_flags, uint32
  * unregister takes the exact pointer that was registered (-ENOENT
  * otherwise) and must come before the memory is freed.  Register memory the
  * caller owns page by page -- DPDK hugepages, an mmap -- not a sub-range of a
- * malloc heap block. */
+ * malloc heap block: its first and last pages hold other objects.
+ *
+ * Registration is optional.  Some systems do not page-lock memory that already
+ * exists: register then returns -ENOTSUP (-ENOMEM: not enough lockable memory;
+ * -EEXIST: locked by other code), nothing is registered, and the _host calls
+ * on that memory take the staged way, with the same results. */
 int mi_cksum_host_register(void *p, uint64_t bytes);
 int mi_cksum_host_unregister(void *p);
 

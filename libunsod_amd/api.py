@@ -532,7 +532,9 @@ def rx_offload_host(buf: np.ndarray, n: int, *, offs=None, stride: int = 0, firs
 def host_register(buf: np.ndarray) -> None:
     """mi_cksum_host_register.  Register memory owned page by page (e.g.
     ``page_buffer``), never a view into a malloc heap block that Python may
-    free and reuse while the pages are locked."""
+    free and reuse while the pages are locked.  Raises MiCksumError with
+    ``rc == -errno.ENOTSUP`` where the system does not page-lock memory that
+    already exists: the ``_host`` calls on it then go the staged way."""
     check("mi_cksum_host_register", load().mi_cksum_host_register(buf.ctypes.data, buf.nbytes))
 
 

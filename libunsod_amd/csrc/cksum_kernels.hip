@@ -5159,7 +5159,13 @@ int mi_cksum_host_register(void *p, uint64_t bytes) {
   if (k >= 0)
     return set_err(-EEXIST, "mi_cksum_host_register: [%p, +%llu) shares a page with the range registered at %p",
                    p, (unsigned long long)bytes, (void *)g_reg[(size_t)k].p);
-  HIP_TRY(hipHostRegister(p, bytes, hipHostRegisterMapped | hipHostRegisterPortable));
+  const hipError_t e = cleared(hipHostRegister(p, bytes, hipHostRegisterMapped | hipHostRegisterPortable));
+  if (e != hipSuccess)  // (a range that is not page-locked: its batches go the staged way)
+    return set_err(e == hipErrorOutOfMemory                  ? -ENOMEM
+                   : e == hipErrorHostMemoryAlreadyRegistered ? -EEXIST
+                                                              : -ENOTSUP,
+                   "mi_cksum_host_register: hipHostRegister(%p, %llu): %s", p, (unsigned long long)bytes,
+                   hipGetErrorString(e));
   jnote("host register", p, bytes);
   jnote("host register pages", (const void *)lo, hi - lo);
   dbg_mem("host-register", p, bytes);

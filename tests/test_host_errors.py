@@ -358,3 +358,26 @@ t.join()
 # first call: staging, then the block, refused: no kernel; second: the block again, a kernel
 assert seen == [(2, 0), (1, 1)], seen
 ''')
+
+
+def test_a_refused_registration_leaves_the_staged_way(so):
+    """Page-locking refused: a distinct code and a clean state, and the batch
+    that follows is verified through staging."""
+    stubbed.run(so, r'''
+n = 64
+b = batch(n)
+o16, o8 = np.zeros(2 * n, np.uint16), np.zeros(n, np.uint8)
+verify = lambda: lib.mi_cksum_ipv4_verify_host(C.byref(b), o16.ctypes.data, None, o8.ctypes.data, None)
+for code, want in ((INVALID, -95), (NOMEM, ENOMEM), (712, -17)):  # 712: hipErrorHostMemoryAlreadyRegistered
+    fail("hipHostRegister", err=code)
+    assert lib.mi_cksum_host_register(b.base, b.bytes) == want, err()
+    assert "hipHostRegister" in err() and stub.stub_last() == 0
+    assert lib.mi__reg_table_count() == 0 and lib.mi_cksum_host_unregister(b.base) == -2
+    before = calls("hipMemcpy2DAsync")
+    assert verify() == 0, err()
+    assert calls("hipMemcpy2DAsync") > before  # staged
+assert lib.mi_cksum_host_register(b.base, b.bytes) == 0, err()
+before = calls("hipMemcpy2DAsync")
+assert verify() == 0 and calls("hipMemcpy2DAsync") == before  # in place
+assert lib.mi_cksum_host_unregister(b.base) == 0 and stub.stub_registered() == 0
+''')
