@@ -828,6 +828,8 @@ def host_path(mi, host: np.ndarray, n: int, L_sum: int, lay: dict, iters: int = 
     kernel reads the registered host batch in place over PCIe); ``staged`` is
     the chunked H2D -> verify -> D2H path on the same bytes."""
     pinned = True
+    host, packets = mi.page_buffer(host.nbytes), host
+    host[:] = packets
     try:
         mi.host_register(host)
     except mi.MiCksumError as e:

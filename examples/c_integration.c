@@ -9,15 +9,13 @@
  *      application threads and the callout thread concurrently), folded on
  *      the CPU (the default) and through the GPU drop-in service.
  *   2. (b2) a host-memory RX burst as the DPDK driver holds it (rte_mbuf slots
- *      of 2176 B, IP header at +142): TX-finalized, registered and verified in
- *      place over PCIe (staged where registration is not supported), then one
- *      corrupted datagram detected.
+ *      of 2176 B, IP header at +142): TX-finalized, registered, verified in
+ *      place over PCIe, then one corrupted datagram detected.
  *
  * Built by libunsod_amd/csrc/Makefile (into libunsod_amd/lib/) with plain gcc:
  *   gcc -O2 -pthread -Iinclude examples/c_integration.c -Llibunsod_amd/lib -lmicksum
  * Prints "c_integration ok" and exits 0 when every check holds.
  */
-#include <errno.h>
 #include <pthread.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -138,9 +136,11 @@ int main(void)
 	const uint32_t n = 1024, L = 1500, stride = 2176, first = 142;
 	const uint64_t bytes = (uint64_t)first + (uint64_t)(n - 1) * stride + L + 64;
 	const uint64_t alloc = (bytes + 4095) & ~4095ull;
-	uint8_t *pool = aligned_alloc(4096, alloc);
-	CHECK(pool != NULL, "alloc");
-	memset(pool, 0, alloc);
+	void *block = NULL; /* page-locked and mapped from the start, zero-filled */
+	CHECK(mi_cksum_host_alloc(alloc, &block) == 0, "host_alloc: %s", mi_cksum_strerror());
+	if (block == NULL)
+		return 1;
+	uint8_t *pool = block;
 	for (uint32_t i = 0; i < n; i++) {
 		uint8_t *ip = pool + first + (uint64_t)i * stride;
 		for (uint32_t k = 40; k < L; k++)
@@ -179,20 +179,18 @@ int main(void)
 	uint16_t *ip_sum = calloc(n, 2), *l4_sum = calloc(n, 2);
 	uint8_t *status = calloc(n, 1);
 	uint32_t bad = 0;
-	/* page-lock + map the pool once: the verify kernel then reads it in place.
-	 * Where the system does not lock memory that already exists (-ENOTSUP) the
-	 * same calls copy the burst through device staging. */
-	const int reg = mi_cksum_host_register(pool, alloc);
-	CHECK(reg == 0 || reg == -ENOTSUP, "register: %s", mi_cksum_strerror());
-	printf("burst: %s\n", reg == 0 ? "read in place" : "staged");
+	/* register the pool once: the verify kernel then reads it in place.  (A pool
+	 * that already exists, DPDK's hugepages, is registered the same way; where
+	 * the system does not lock such memory, -ENOTSUP, the same calls copy the
+	 * burst through device staging.) */
+	CHECK(mi_cksum_host_register(pool, alloc) == 0, "register: %s", mi_cksum_strerror());
 	CHECK(mi_cksum_ipv4_verify_host(&b, ip_sum, l4_sum, status, &bad) == 0, "verify_host: %s", mi_cksum_strerror());
 	CHECK(bad == 0, "valid burst: %u bad", bad);
 	pool[first + 777u * stride + 900] ^= 0x10;
 	CHECK(mi_cksum_ipv4_verify_host(&b, ip_sum, l4_sum, status, &bad) == 0, "verify_host: %s", mi_cksum_strerror());
 	CHECK(bad == 1 && status[777] == MI_ST_L4_BAD, "corrupted datagram: bad %u status %u", bad, status[777]);
-	if (reg == 0)
-		CHECK(mi_cksum_host_unregister(pool) == 0, "unregister: %s", mi_cksum_strerror());
-	free(pool);
+	CHECK(mi_cksum_host_unregister(pool) == 0, "unregister: %s", mi_cksum_strerror());
+	CHECK(mi_cksum_host_free(pool) == 0, "host_free: %s", mi_cksum_strerror());
 	free(ip_sum);
 	free(l4_sum);
 	free(status);

@@ -546,6 +546,17 @@ int mi_cksum_rx_offload_host(const mi_pkt_batch *b, uint32_t *csum_flags, uint32
 int mi_cksum_host_register(void *p, uint64_t bytes);
 int mi_cksum_host_unregister(void *p);
 
+/* Host memory that is page-locked and mapped from the start (hipHostMalloc):
+ * *out = a page-aligned, zero-filled block of at least `bytes`, for a packet
+ * pool whose owner can choose where it lies.  A range inside the block is
+ * registered and unregistered as above, at no cost and on every system; one
+ * that reaches past the block is refused (-EINVAL).  -ENOMEM: not enough
+ * memory.  host_free takes the pointer host_alloc gave (-ENOENT otherwise; NULL
+ * is nothing), once every call that uses the block has returned and its ranges
+ * are unregistered (-EBUSY: the block stays). */
+int mi_cksum_host_alloc(uint64_t bytes, void **out);
+int mi_cksum_host_free(void *p);
+
 /* ------------------------------------------------------------------------ */
 /* workload generator (bench / tests; not part of the reference API)          */
 /* ------------------------------------------------------------------------ */

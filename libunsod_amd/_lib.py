@@ -164,6 +164,8 @@ SIGNATURES = {
     "mi_cksum_rx_offload_host": (C.c_int, [C.POINTER(PktBatchC), C.c_void_p, C.c_void_p, C.c_void_p]),
     "mi_cksum_host_register": (C.c_int, [C.c_void_p, C.c_uint64]),
     "mi_cksum_host_unregister": (C.c_int, [C.c_void_p]),
+    "mi_cksum_host_alloc": (C.c_int, [C.c_uint64, C.POINTER(C.c_void_p)]),
+    "mi_cksum_host_free": (C.c_int, [C.c_void_p]),
     "mi_cksum_synth_ipv4": (C.c_int, [C.POINTER(PktBatchC), C.c_uint64, C.c_void_p]),
     "mi_cksum_hsa_queues": (C.c_int, []),
     "mi_cksum_set_dropin_error_handler": (None, [C.c_void_p]),

@@ -13,6 +13,7 @@ kernels on the current torch stream (asynchronous).
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 from typing import Iterable
 
 import numpy as np
@@ -539,10 +540,18 @@ def host_register(buf: np.ndarray) -> None:
 
 
 def page_buffer(nbytes: int) -> np.ndarray:
-    """A uint8 array of ``nbytes`` on pages of its own: an anonymous mmap,
-    page-aligned, that no other object shares and that malloc never hands
-    out again -- what host_register should be given (the role DPDK's
-    hugepage memory plays for the reference's mbufs)."""
+    """A uint8 array of ``nbytes`` zeros on pages of its own, page-aligned, that
+    no other object shares -- what host_register should be given (the role
+    DPDK's hugepage memory plays for the reference's mbufs).  With a device it
+    is a block of mi_cksum_host_alloc, registrable on every system and freed
+    with the last array over it (kept if a range of it is still registered);
+    without one, an anonymous mmap."""
+    if device_count() > 0:
+        lib, p = load(), C.c_void_p()
+        check("mi_cksum_host_alloc", lib.mi_cksum_host_alloc(max(1, nbytes), C.byref(p)))
+        block = (C.c_uint8 * max(1, nbytes)).from_address(p.value)
+        weakref.finalize(block, lib.mi_cksum_host_free, p.value).atexit = False
+        return np.frombuffer(block, np.uint8, count=nbytes)
     import mmap
     m = mmap.mmap(-1, max(1, (nbytes + 4095) & ~4095))
     return np.frombuffer(m, np.uint8, count=nbytes)

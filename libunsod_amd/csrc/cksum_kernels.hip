@@ -5118,6 +5118,21 @@ struct HostRange {
 };
 static std::mutex g_reg_mu;
 static std::vector<HostRange> g_reg;
+// Blocks of mi_cksum_host_alloc: page-locked and mapped from the start, so a
+// range inside one is registered by its table entry alone, without the runtime
+// (which does not lock memory that is locked already, and on some systems no
+// memory that already exists).
+struct HostBlock {
+  uintptr_t lo, hi;  // whole pages
+  uintptr_t dev;     // the GPU address of lo
+};
+static std::vector<HostBlock> g_blocks;  // (under g_reg_mu)
+// g_reg_mu held: the block that overlaps [lo, hi), or -1.
+static long block_overlap(uintptr_t lo, uintptr_t hi) {
+  for (size_t k = 0; k < g_blocks.size(); ++k)
+    if (lo < g_blocks[k].hi && hi > g_blocks[k].lo) return (long)k;
+  return -1;
+}
 
 static void reg_pages(const void *p, uint64_t bytes, uintptr_t *lo, uintptr_t *hi) {
   *lo = (uintptr_t)p & ~(uintptr_t)4095;
@@ -5159,6 +5174,15 @@ int mi_cksum_host_register(void *p, uint64_t bytes) {
   if (k >= 0)
     return set_err(-EEXIST, "mi_cksum_host_register: [%p, +%llu) shares a page with the range registered at %p",
                    p, (unsigned long long)bytes, (void *)g_reg[(size_t)k].p);
+  if (const long j = block_overlap(lo, hi); j >= 0) {
+    const HostBlock &blk = g_blocks[(size_t)j];
+    if (lo < blk.lo || hi > blk.hi)
+      return set_err(-EINVAL, "mi_cksum_host_register: [%p, +%llu) reaches past the mi_cksum_host_alloc block at %p", p,
+                     (unsigned long long)bytes, (void *)blk.lo);
+    g_reg.push_back({lo, hi, (uintptr_t)p, blk.dev + ((uintptr_t)p - blk.lo)});
+    jnote("host register (own block)", p, bytes);
+    return 0;
+  }
   const hipError_t e = cleared(hipHostRegister(p, bytes, hipHostRegisterMapped | hipHostRegisterPortable));
   if (e != hipSuccess)  // (a range that is not page-locked: its batches go the staged way)
     return set_err(e == hipErrorOutOfMemory                  ? -ENOMEM
@@ -5187,10 +5211,55 @@ int mi_cksum_host_unregister(void *p) {
     lo = g_reg[(size_t)k].lo;
     hi = g_reg[(size_t)k].hi;
     g_reg.erase(g_reg.begin() + k);
+    if (block_overlap(lo, hi) >= 0) {  // (stays locked and mapped: its block's)
+      jnote("host unregister (own block)", p, hi - lo);
+      return 0;
+    }
   }
   dbg_mem("host-unregister", p, 0);
   jnote("host unregister pages", (const void *)lo, hi - lo);
   HIP_TRY(hipHostUnregister(p));
+  return 0;
+}
+
+int mi_cksum_host_alloc(uint64_t bytes, void **out) {
+  if (!out) return set_err(-EINVAL, "mi_cksum_host_alloc: out is NULL");
+  *out = nullptr;
+  if (!bytes || bytes > UINT64_MAX - 4095) return set_err(-EINVAL, "mi_cksum_host_alloc: %llu bytes", (unsigned long long)bytes);
+  int rc = ensure_ctx();
+  if (rc) return rc;
+  const uint64_t n = (bytes + 4095) & ~4095ull;
+  void *p = nullptr, *dev = nullptr;
+  // (coherent: the host writes packets here between calls and the kernels write
+  // TX slots, with no copy in between that would make them visible)
+  const hipError_t e = jhostmalloc(&p, n, hipHostMallocMapped | hipHostMallocPortable | hipHostMallocCoherent);
+  if (e != hipSuccess)
+    return set_err(-ENOMEM, "mi_cksum_host_alloc: %llu bytes: %s", (unsigned long long)n, hipGetErrorString(e));
+  if (cleared(hipHostGetDevicePointer(&dev, p, 0)) != hipSuccess || !dev || ((uintptr_t)p & 4095)) {
+    (void)jhostfree(p);
+    return set_err(-EIO, "mi_cksum_host_alloc: no page-aligned block with a device address");
+  }
+  memset(p, 0, n);
+  dbg_mem("host-alloc", p, n);
+  std::lock_guard<std::mutex> g(g_reg_mu);
+  g_blocks.push_back({(uintptr_t)p, (uintptr_t)p + n, (uintptr_t)dev});
+  *out = p;
+  return 0;
+}
+
+int mi_cksum_host_free(void *p) {
+  if (!p) return 0;
+  {
+    std::lock_guard<std::mutex> g(g_reg_mu);
+    size_t j = 0;
+    while (j < g_blocks.size() && g_blocks[j].lo != (uintptr_t)p) ++j;
+    if (j == g_blocks.size()) return set_err(-ENOENT, "mi_cksum_host_free: %p is not a block of mi_cksum_host_alloc", p);
+    if (const long k = reg_overlap(g_blocks[j].lo, g_blocks[j].hi); k >= 0)
+      return set_err(-EBUSY, "mi_cksum_host_free: the range at %p is still registered", (void *)g_reg[(size_t)k].p);
+    g_blocks.erase(g_blocks.begin() + (long)j);
+  }
+  dbg_mem("host-free", p, 0);
+  HIP_TRY(jhostfree(p));
   return 0;
 }
 

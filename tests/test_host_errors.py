@@ -381,3 +381,109 @@ before = calls("hipMemcpy2DAsync")
 assert verify() == 0 and calls("hipMemcpy2DAsync") == before  # in place
 assert lib.mi_cksum_host_unregister(b.base) == 0 and stub.stub_registered() == 0
 ''')
+
+
+def test_host_blocks(so):
+    """mi_cksum_host_alloc: zero-filled pages whose ranges are registered without
+    the runtime, read in place while they are and staged after; the refusals; no
+    block is freed under a registered range or leaked by a failed call."""
+    stubbed.run(so, r'''
+EINVAL, ENOENT, EBUSY, EEXIST = -22, -2, -16, -17
+p = C.c_void_p()
+
+
+def alloc(n):
+    p = C.c_void_p(1)
+    rc = lib.mi_cksum_host_alloc(n, C.byref(p))
+    return rc, p.value or 0
+
+
+assert lib.mi_cksum_host_alloc(4096, None) == EINVAL
+for bad in (0, 2**64 - 1, 2**64 - 4095):
+    assert alloc(bad) == (EINVAL, 0), bad
+live = stub.stub_live()
+fail("hipHostMalloc", err=NOMEM)
+assert alloc(4096) == (ENOMEM, 0)
+fail("hipHostGetDevicePointer")
+assert alloc(4096) == (EIO, 0) and stub.stub_live() == live and stub.stub_last() == 0
+assert lib.mi_cksum_host_free(None) == 0 and lib.mi_cksum_host_free(4096) == ENOENT
+
+n = 64
+size = 142 + n * 2176 + 64
+rc, a = alloc(size)
+assert rc == 0 and a % 4096 == 0
+assert not np.ctypeslib.as_array((C.c_uint8 * size).from_address(a)).any()
+end = a + ((size + 4095) & ~4095)
+b = _lib.PktBatchC(a, size, None, 2176, 142, None, 1500, n, 1500, 0)
+st = np.zeros(n, np.uint8)
+
+
+def staged():  # does a verify of the block go through staging?
+    before = calls("hipMemcpy2DAsync")
+    assert lib.mi_cksum_ipv4_verify_host(C.byref(b), None, None, st.ctypes.data, None) == 0, err()
+    return calls("hipMemcpy2DAsync") > before
+
+
+assert staged()  # a block is not a registered range
+assert lib.mi_cksum_host_register(a, end - a + 1) == EINVAL  # one byte past the block's last page
+assert lib.mi_cksum_host_register(a - 1, 4096) == EINVAL
+assert lib.mi__reg_table_count() == 0 and staged()
+assert lib.mi_cksum_host_register(a, size) == 0 and not staged()
+assert lib.mi_cksum_host_register(a + 4096, 10) == EEXIST
+assert lib.mi_cksum_host_free(a) == EBUSY and lib.mi_cksum_host_free(a + 4096) == ENOENT
+assert not staged()  # still there
+assert lib.mi_cksum_host_unregister(a + 1) == ENOENT and lib.mi_cksum_host_unregister(a) == 0
+assert staged() and lib.mi_cksum_host_unregister(a) == ENOENT
+# two ranges of one block, pages apart; the GPU address is the block's plus the offset
+lib.mi__reg_table_lookup.restype, lib.mi__reg_table_lookup.argtypes = C.c_uint64, [C.c_void_p, C.c_uint64]
+assert lib.mi_cksum_host_register(a, 4096) == 0 and lib.mi_cksum_host_register(a + 8192 + 32, 100) == 0
+assert lib.mi__reg_table_lookup(a + 16, 64) == a + 16 and lib.mi__reg_table_lookup(a + 8192 + 64, 32) == a + 8192 + 64
+assert lib.mi__reg_table_lookup(a + 4096, 16) == 0
+assert lib.mi_cksum_host_unregister(a) == 0 and lib.mi_cksum_host_free(a) == EBUSY
+assert lib.mi_cksum_host_unregister(a + 8192 + 32) == 0
+assert calls("hipHostRegister") == calls("hipHostUnregister") == 0
+live = stub.stub_live()
+assert lib.mi_cksum_host_free(a) == 0 and stub.stub_live() == live - 1
+assert lib.mi_cksum_host_free(a) == ENOENT and stub.stub_bad_frees() == 0
+''')
+
+
+def test_page_buffer_frees_its_block(so):
+    """mi.page_buffer with a device: the block goes with the last array over it,
+    not while a view lives or a range is registered."""
+    stubbed.run(so, r'''
+import gc
+import types
+
+# the package's api module over the stubbed library
+pkg = types.ModuleType("libunsod_amd")
+pkg.__path__ = [os.path.join(ROOT, "libunsod_amd")]
+sys.modules["libunsod_amd"] = pkg
+sys.modules["libunsod_amd._lib"] = _lib
+_lib._lib = lib
+import importlib
+api = importlib.import_module("libunsod_amd.api")
+
+live = stub.stub_live()
+a = api.page_buffer(5000)
+assert a.nbytes == 5000 and a.ctypes.data % 4096 == 0 and a.flags.writeable and not a.any()
+assert stub.stub_live() == live + 1
+v = a[100:200].reshape(10, 10)
+del a
+gc.collect()
+v[:] = 7
+assert stub.stub_live() == live + 1
+del v
+gc.collect()
+assert stub.stub_live() == live
+assert api.page_buffer(0).nbytes == 0
+gc.collect()
+assert stub.stub_live() == live
+a = api.page_buffer(100)
+api.host_register(a)
+p = a.ctypes.data
+del a
+gc.collect()
+assert stub.stub_live() == live + 1  # registered: kept
+assert lib.mi_cksum_host_unregister(p) == 0 and lib.mi_cksum_host_free(p) == 0 and stub.stub_live() == live
+''')

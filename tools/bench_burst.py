@@ -70,9 +70,7 @@ def main():
     db = mi.PktBatch(dbuf, nmax, stride=STRIDE, first_off=FIRST, fixed_len=L)
     mi.synth_ipv4(db, seed=0xB0057)
     mi.ipv4_finalize(db)
-    raw = np.zeros(size + 8192, np.uint8)
-    s = (-raw.ctypes.data) % 4096
-    host = raw[s:s + size]
+    host = mi.page_buffer(size)
     host[:] = dbuf.cpu().numpy()
     mi.host_register(host)
     ref = Oracle("reference" if available("reference") else "port")

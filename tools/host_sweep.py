@@ -36,9 +36,7 @@ def main():
     mi.ipv4_finalize(b)
     torch.cuda.synchronize()
     raw = buf.cpu().numpy()
-    host = np.zeros(raw.size + 8192, np.uint8)
-    s = (-host.ctypes.data) % 4096
-    h = host[s:s + raw.size]
+    h = mi.page_buffer(raw.size)
     h[:] = raw
     lay = dict(stride=stride, first_off=first, fixed_len=L)
     mi.host_register(h)

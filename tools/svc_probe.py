@@ -20,9 +20,7 @@ lib.mi__set_dropin_service.argtypes = [C.c_int]
 KAT_HDR = bytes.fromhex("450000730000400040110000c0a80001c0a800c7")
 n, L, stride, first = 200, 1500, 2176, 142
 b = synth.build_ipv4_batch(n, L, stride=stride, first_off=first, seed=3)
-raw = np.zeros(b["buf"].size + 4096, np.uint8)
-s = (-raw.ctypes.data) % 4096
-buf = raw[s:s + b["buf"].size]
+raw = buf = mi.page_buffer(b["buf"].size)
 buf[:] = b["buf"]
 mi.host_register(raw)
 torch.cuda.init()
