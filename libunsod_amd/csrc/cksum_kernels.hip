@@ -6066,11 +6066,11 @@ int mi__spin(uint32_t us, int via) {
 }
 // Diagnostics (tools/queue_place_probe.py): a resident wave for `us`
 // microseconds on the k-th of up to 16 extra queues of the calling thread's
-// device (created in order on first use, 64 packets; prio >= 0: set the
-// queue's priority first, 0 low .. 2 high).
+// device (created in order on first use, 64 packets, default priority: work on
+// queues of different priorities has hung this device).
 static hsa_queue_t *g_spin_qs[16];
 long long mi__spin_queue_id(int k) { return k >= 0 && k < 16 && g_spin_qs[k] ? (long long)g_spin_qs[k]->id : -1; }
-int mi__spin_queue(uint32_t us, int k, int prio) {
+int mi__spin_queue(uint32_t us, int k) {
   hsa_queue_t **qs = g_spin_qs;
   static std::atomic<int> qerr{0};
   if (k < 0 || k >= 16) return set_err(-EINVAL, "queue index");
@@ -6080,8 +6080,6 @@ int mi__spin_queue(uint32_t us, int k, int prio) {
   std::lock_guard<std::mutex> lk(o.dev->dq_mu);
   for (int j = 0; j <= k; ++j)
     if (!qs[j] && (rc = aql_queue_create(o.dev->agent, 64, &qerr, &qs[j]))) return rc;
-  if (prio >= 0 && hsa_amd_queue_set_priority(qs[k], (hsa_amd_queue_priority_t)prio) != HSA_STATUS_SUCCESS)
-    return set_err(-EIO, "hsa_amd_queue_set_priority");
   const uint64_t ticks = (uint64_t)us * 100u;
   uint8_t *ka = o.karg + 512u * (o.next++ % kAqlOneSlots);
   return dq_dispatch_locked(o.dev, qs[k], kAqlSpin, 1, 64, &ticks, sizeof ticks, ka, hsa_signal_t{0});

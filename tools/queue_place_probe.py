@@ -6,8 +6,7 @@ touches no memory cost the 1500 B batch path nothing on a HIP stream or on
 the library's service queue, and 0.65x of its rate on the library's dispatch
 queue -- the same kernel, another queue.  Here 8 extra queues are created in
 order after the batch side's two AQL queues; a resident wave sits on queue k
-(k = 0..7) for 2 s while the batch rate is measured; then again at low and
-high queue priority.  One JSON line per case.
+(k = 0..7) for 2 s while the batch rate is measured.  One JSON line per case.
 
 --foreign N first creates N queues the library does not know of (raw HSA,
 as another component of the process would) between the batch pair and the
@@ -68,13 +67,12 @@ def main():
     import argparse
     ap = argparse.ArgumentParser()
     ap.add_argument("--foreign", type=int, default=0)
-    ap.add_argument("--priorities", default="-1,0,2")
     a = ap.parse_args()
     lib = mi.load()
     lib.mi__spin_queue_id.restype = C.c_longlong
     lib.mi__repeat_queue_id.restype = C.c_longlong
     lib.mi__repeat_queue_id.argtypes = [C.c_void_p, C.c_int]
-    lib.mi__spin_queue.argtypes = [C.c_uint32, C.c_int, C.c_int]
+    lib.mi__spin_queue.argtypes = [C.c_uint32, C.c_int]
     lib.mi__set_dropin_service.argtypes = [C.c_int]
     lib.mi__set_dropin_service(0)
     lib.mi_cksum_hsa_queues.restype = C.c_int
@@ -104,16 +102,15 @@ def main():
     fq = foreign_queues(a.foreign) if a.foreign else []
     print(json.dumps(dict(case="none", batch_gib_s=base, library_queues=lib.mi_cksum_hsa_queues(),
                           batch_queue_ids=[ida, idb], foreign_queues=len(fq))), flush=True)
-    for prio in [int(x) for x in a.priorities.split(",")]:
-        for k in range(8):
-            assert lib.mi__spin_queue(1_600_000, k, prio) == 0
-            time.sleep(0.1)
-            r = rate()
-            qid = lib.mi__spin_queue_id(k)
-            print(json.dumps(dict(case="resident wave", queue=k, queue_id=qid, priority=prio, batch_gib_s=r,
-                                  batch_vs_none=round(r / base, 3),
-                                  id_rule_shared_pipe=(qid - ida) % 4 in (0, 1))), flush=True)
-            time.sleep(0.5)
+    for k in range(8):
+        assert lib.mi__spin_queue(1_600_000, k) == 0
+        time.sleep(0.1)
+        r = rate()
+        qid = lib.mi__spin_queue_id(k)
+        print(json.dumps(dict(case="resident wave", queue=k, queue_id=qid, batch_gib_s=r,
+                              batch_vs_none=round(r / base, 3),
+                              id_rule_shared_pipe=(qid - ida) % 4 in (0, 1))), flush=True)
+        time.sleep(0.5)
     rep.close()
 
 
