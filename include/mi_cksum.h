@@ -146,6 +146,10 @@ int mi_cksum_set_run_kernel(int chunks, int slots);
  *             correctly (per-datagram fallback), only slower.
  * Spans outside [0, bytes) read as zero bytes (hardware bounds check), never
  * fault.
+ * A call on `stream` that returns an error may have enqueued part of its work
+ * (a batch of several launches): synchronize the stream before freeing what it
+ * was given.  The synchronous calls (the _host ones, back-to-back submissions,
+ * handle runs) leave nothing running behind an error.
  */
 #define MI_BATCH_MAX_BYTES 0xFFFFE000ull
 /* At most this many packets (spans, chains, frames) per batch: every
@@ -553,7 +557,8 @@ int mi_cksum_host_unregister(void *p);
  * that reaches past the block is refused (-EINVAL).  -ENOMEM: not enough
  * memory.  host_free takes the pointer host_alloc gave (-ENOENT otherwise; NULL
  * is nothing), once every call that uses the block has returned and its ranges
- * are unregistered (-EBUSY: the block stays). */
+ * are unregistered (-EBUSY: the block stays).  Neither may run while a stream of
+ * the process is captured in the global mode (hipHostMalloc, hipHostFree). */
 int mi_cksum_host_alloc(uint64_t bytes, void **out);
 int mi_cksum_host_free(void *p);
 

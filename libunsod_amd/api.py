@@ -13,6 +13,7 @@ kernels on the current torch stream (asynchronous).
 from __future__ import annotations
 
 import ctypes as C
+import errno
 import weakref
 from typing import Iterable
 
@@ -545,10 +546,11 @@ def page_buffer(nbytes: int) -> np.ndarray:
     DPDK's hugepage memory plays for the reference's mbufs).  With a device it
     is a block of mi_cksum_host_alloc, registrable on every system and freed
     with the last array over it (kept if a range of it is still registered);
-    without one, an anonymous mmap."""
-    if device_count() > 0:
-        lib, p = load(), C.c_void_p()
-        check("mi_cksum_host_alloc", lib.mi_cksum_host_alloc(max(1, nbytes), C.byref(p)))
+    without a usable one, an anonymous mmap."""
+    lib, p = load(), C.c_void_p()
+    rc = lib.mi_cksum_host_alloc(max(1, nbytes), C.byref(p))
+    if rc != -errno.ENODEV:
+        check("mi_cksum_host_alloc", rc)
         block = (C.c_uint8 * max(1, nbytes)).from_address(p.value)
         weakref.finalize(block, lib.mi_cksum_host_free, p.value).atexit = False
         return np.frombuffer(block, np.uint8, count=nbytes)

@@ -486,4 +486,8 @@ del a
 gc.collect()
 assert stub.stub_live() == live + 1  # registered: kept
 assert lib.mi_cksum_host_unregister(p) == 0 and lib.mi_cksum_host_free(p) == 0 and stub.stub_live() == live
+stub.stub_fail_from(b"hipGetDevice", 1, 100)  # no usable device: pages of its own all the same
+allocs = calls("hipHostMalloc")
+a = api.page_buffer(5000)
+assert a.nbytes == 5000 and a.ctypes.data % 4096 == 0 and a.flags.writeable and calls("hipHostMalloc") == allocs
 ''')
