@@ -149,7 +149,8 @@ int mi_cksum_set_run_kernel(int chunks, int slots);
  * A call on `stream` that returns an error may have enqueued part of its work
  * (a batch of several launches): synchronize the stream before freeing what it
  * was given.  The synchronous calls (the _host ones, back-to-back submissions,
- * handle runs) leave nothing running behind an error.
+ * handle runs) leave nothing running behind an error, unless the error is that
+ * the work did not end: no result within 10 s, or a device that failed.
  */
 #define MI_BATCH_MAX_BYTES 0xFFFFE000ull
 /* At most this many packets (spans, chains, frames) per batch: every
